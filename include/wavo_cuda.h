@@ -335,6 +335,122 @@ wavo_status wavo_pick(wavo_ctx *ctx, float *logits, uint32_t ld, uint32_t rows, 
                       uint32_t no_timestamps, uint32_t begin, uint32_t max_initial,
                       int32_t *tokens, float *logprobs);
 
+/* ---- paged caches and drafted trees: a decode step that verifies several tokens -------------
+ * No reference counterparts: the reference keeps one contiguous cache a window and decodes a token
+ * a step (src/transformer.rs:254-290).
+ *
+ * A paged cache ("pool", device, 16-byte aligned) holds `blocks` blocks of bs positions in f16,
+ * [blocks][K, V][kv_heads][bs][hd]; a slot is block * bs + offset. bs is a power of two from 8 to
+ * 256, hd a multiple of 8 up to 128, blocks * bs < 2^31. Block tables are [n][width] block ids:
+ * position p of request s is in block table[s][p / bs].
+ *
+ * The rows of a step are those of its n requests one after another: request s has the rows
+ * row_start[s] .. row_start[s + 1]. With drafted tokens they form a tree: row 0 of a request is the
+ * last token decided, the others drafted continuations, parents before children. Row i's mask
+ * words (bit j % 32 of word j / 32 is row j of the request) hold its path: its ancestors and itself.
+ * Row j's K and V are at position len + j. */
+
+/* Block tables and the slot map of a step from the requests' lengths. Request s holds lens[s]
+ * positions in owned[s] blocks (its table's first entries) and brings adds[s] rows; adds[s] < 0: it
+ * is done and gives its blocks back. Free block ids are a ring of ring_cap ids, state[0] the index of
+ * the first, state[1] how many. Requests take the blocks they lack, in order, while they last: a
+ * request is refused when the blocks lacking up to and with its own exceed those free, or when it
+ * needs more than `width`; it then keeps what it has and its rows get no slots. A request that
+ * lacks none is always served. Blocks given back can be taken from the next call on.
+ * Out: the tables' new entries; owned_out; row_start [n + 1] (all requests' rows, refused ones'
+ * too); for rows below rows_cap row_seq (the request) and slots, both -1 past the last row, slots
+ * -1 for refused requests; state_out: the ring's new state, the number of rows, the number of
+ * requests refused. state_out and owned_out must not be state and owned (EINVAL): a step that is
+ * run again on the same inputs gives the same outputs. n * width < 2^31. */
+wavo_status wavo_block_tables(wavo_ctx *ctx, const int32_t *lens, const int32_t *adds, uint32_t n,
+                              uint32_t bs, int32_t *ring, uint32_t ring_cap, const int32_t *state,
+                              const int32_t *owned, int32_t *table, uint32_t width,
+                              int32_t *row_start, int32_t *row_seq, int32_t *slots,
+                              uint32_t rows_cap, int32_t *state_out, int32_t *owned_out);
+
+/* wavo_pack for a paged cache: rows rows of x (x_dtype) from element src on, `stride` elements
+ * apart, each K then V of kv_heads * hd values, rounded to f16 into their slots. Rows whose slot is
+ * not in the pool (-1) are skipped; two rows with one slot are not ordered. */
+wavo_status wavo_pack_slots(wavo_ctx *ctx, const void *x, int x_dtype, uint32_t src,
+                            uint32_t stride, const int32_t *slots, uint32_t rows, void *pool,
+                            uint32_t blocks, uint32_t bs, uint32_t kv_heads, uint32_t hd);
+
+/* Attention of `rows` rows q [rows][heads * hd] (row stride q_stride elements; 0: heads * hd) of n
+ * requests over a paged cache into o (o_stride likewise), both of `dtype`. A row sees its request's
+ * positions 0 .. lens[s] and, with a mask ([rows][mask_words], mask_words <= 8), the positions
+ * lens[s] + j of the rows j < the request's whose bit is set; any bits may be set. mask NULL: the
+ * lens[s] positions alone (a single token whose K and V are packed already, or the queries of a
+ * cross attention over the encoder frames). row_start NULL: request s has the one row s. Head h reads
+ * K and V head h / (heads / kv_heads). max_rows is at least the rows of every request (at most
+ * 32 * mask_words with a mask), max_len at least every number of positions. Scores are scaled by
+ * 1 / sqrt(hd). A row that sees nothing gets zeros; what a row does not see has no effect on it,
+ * whatever it holds. WAVO_F16: f16 products, f32 sums, probabilities rounded to f16 before they
+ * meet V. WAVO_F32: q and the probabilities enter as two f16 parts each, f32 accuracy (q below
+ * f16's largest value). Table entries outside the pool are positions that no row sees.
+ * wavo_attend_tree_scratch is the scratch that a call needs (see wavo_reserve). */
+wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, int dtype,
+                             const void *pool, uint32_t blocks, uint32_t bs, const int32_t *table,
+                             uint32_t width, const int32_t *row_start, const int32_t *lens,
+                             uint32_t n, const uint32_t *mask, uint32_t mask_words, uint32_t rows,
+                             uint32_t max_rows, uint32_t max_len, void *o, uint64_t o_stride,
+                             uint32_t heads, uint32_t kv_heads, uint32_t hd);
+size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t n, uint32_t rows, uint32_t max_rows,
+                                uint32_t max_len, uint32_t heads, uint32_t kv_heads, uint32_t hd);
+
+/* What wavo_shape_logits applies to a row of a request, each part off where its pointers are NULL.
+ * Device buffers; the struct itself is read at the call. */
+typedef struct wavo_logit_rules {
+  uint32_t vocab, n;         /* tokens; requests */
+  const int32_t *row_seq;    /* [rows] the row's request, -1: padding; NULL: row r is request r */
+  /* The tokens before a row: its request's history [n][max_hist], hist_len[s] of it, and the drafted
+   * tokens on its path: tokens[row_start[s] + j] for the bits j of path [rows][path_words], the
+   * row's own among them. Ids outside the vocabulary do not count. max_hist + 32 * path_words
+   * <= 65535. */
+  const int32_t *history, *hist_len;
+  uint32_t max_hist;
+  const int32_t *row_start, *tokens;
+  const uint32_t *path;
+  uint32_t path_words;
+  /* [n][3] f32: repetition, presence, frequency. A token that is among them c > 0 times: x > 0 is
+   * divided by repetition, else multiplied; then frequency * c + presence is subtracted. */
+  const float *penalties;
+  /* [n][max_bias] ids and values, bias_len[s] of them: added to their tokens (finite, or -inf). Of an
+   * id's entries the last holds. max_bias <= 65534. */
+  const int32_t *bias_ids;
+  const float *bias_vals;
+  const int32_t *bias_len;
+  uint32_t max_bias;
+  /* n_grammar sets of allowed tokens, bit t % 32 of word t / 32, grammar_ld words apart, and each
+   * row's set (grammar_of [rows]; -1: all tokens are allowed). Others get -inf. */
+  const uint32_t *grammar;
+  uint32_t n_grammar, grammar_ld;
+  const int32_t *grammar_of;
+} wavo_logit_rules;
+
+/* logits [rows][vocab] (dtype, row stride ld; 0: vocab) edited by the rules (penalties, biases,
+ * grammar, in this order, each step rounded in f32) into `out` (same dtype; may be logits; NULL: not
+ * wanted), and of the edited values, before they are rounded to dtype, the first maximum (picks
+ * [rows]) and its log-softmax (logprobs [rows]); either may be NULL. A row that is left with -inf
+ * alone, and padding, get pick -1 and logprob -inf; padding's `out` row is left as it is. NaN is
+ * never picked, and makes its row's logprob NaN. */
+wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint64_t ld, void *out,
+                              uint64_t ld_out, uint32_t rows, const wavo_logit_rules *rules,
+                              int32_t *picks, float *logprobs);
+
+/* The drafted path that the picks confirm, and its place in the cache: from a request's row 0 to
+ * the first child (a row whose path is the node's and itself) whose token is the node's pick, as
+ * far as that goes. path [n][max_rows] gets the nodes, then -1; count [n] how many (0 for a request
+ * without rows); next [n] the last node's pick (-1 without rows); new_lens[s] = lens[s] + count (not
+ * the same buffer as lens: EINVAL). With a pool of `layers` layers, layer_stride elements apart, the
+ * K and V of node path[k] move to position lens[s] + k in each. max_rows <= 256, mask_words <= 8. */
+wavo_status wavo_tree_accept(wavo_ctx *ctx, const int32_t *picks, const int32_t *tokens,
+                             const uint32_t *mask, uint32_t mask_words, uint32_t rows,
+                             const int32_t *row_start, uint32_t n, uint32_t max_rows,
+                             const int32_t *lens, const int32_t *table, uint32_t width, void *pool,
+                             uint32_t layers, uint64_t layer_stride, uint32_t blocks, uint32_t bs,
+                             uint32_t kv_heads, uint32_t hd, int32_t *path, int32_t *count,
+                             int32_t *next, int32_t *new_lens);
+
 /* pos_rows (src/gpu/mod.rs:1060-1065): 2t + 15. */
 uint32_t wavo_pos_rows(uint32_t t);
 

@@ -26,6 +26,17 @@ _vp, _u32, _u64, _i32, _f32, _sz = (ctypes.c_void_p, ctypes.c_uint32, ctypes.c_u
                                     ctypes.c_int, ctypes.c_float, ctypes.c_size_t)
 _st = ctypes.c_int
 
+
+class LogitRulesC(ctypes.Structure):
+    """wavo_logit_rules."""
+    _fields_ = [
+        ("vocab", _u32), ("n", _u32), ("row_seq", _vp), ("history", _vp), ("hist_len", _vp),
+        ("max_hist", _u32), ("row_start", _vp), ("tokens", _vp), ("path", _vp),
+        ("path_words", _u32), ("penalties", _vp), ("bias_ids", _vp), ("bias_vals", _vp),
+        ("bias_len", _vp), ("max_bias", _u32), ("grammar", _vp), ("n_grammar", _u32),
+        ("grammar_ld", _u32), ("grammar_of", _vp)]
+
+
 SIGNATURES = {
     "wavo_device_count": ([], _i32),
     "wavo_create": ([_i32, ctypes.POINTER(_vp)], _st),
@@ -98,6 +109,16 @@ SIGNATURES = {
                            _u32], _st),
     "wavo_attend_batch_noalloc": ([_vp, _u64, _vp, _u64, _vp, _u64, _u32, _u32, _u32, _u32,
                                    _u32, _vp], _st),
+    "wavo_block_tables": ([_vp, _vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _u32, _vp, _vp,
+                           _vp, _u32, _vp, _vp], _st),
+    "wavo_pack_slots": ([_vp, _vp, _i32, _u32, _u32, _vp, _u32, _vp, _u32, _u32, _u32, _u32], _st),
+    "wavo_attend_tree": ([_vp, _vp, _u64, _i32, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _u32, _vp,
+                          _u32, _u32, _u32, _u32, _vp, _u64, _u32, _u32, _u32], _st),
+    "wavo_attend_tree_scratch": ([_vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32], _sz),
+    "wavo_shape_logits": ([_vp, _vp, _i32, _u64, _vp, _u64, _u32, ctypes.POINTER(LogitRulesC),
+                           _vp, _vp], _st),
+    "wavo_tree_accept": ([_vp, _vp, _vp, _vp, _u32, _u32, _vp, _u32, _u32, _vp, _vp, _u32, _vp,
+                          _u32, _u64, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp], _st),
     "wavo_capture_begin": ([_vp], _st),
     "wavo_capture_end": ([_vp, ctypes.POINTER(_vp)], _st),
     "wavo_graph_launch": ([_vp, _vp], _st),

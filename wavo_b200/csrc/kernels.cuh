@@ -183,6 +183,89 @@ cudaError_t launch_gemv(const float *a, long long lda, int wtype, const void *w,
                         const float *scales, const float *bias, float *c, long long ldc, int rows,
                         int n, int k, int epilogue, float alpha, cudaStream_t s);
 
+// ---- paged caches and drafted trees (paged.cu, tree.cu, shape.cu) ------------------------------
+
+struct BlockTablesArgs {
+  const int *lens, *adds;  // [n]: positions held; rows of this step, negative: the request is done
+  int n, bs;
+  int *ring;               // ids of free blocks, `cap` of them, used as a ring
+  int cap;
+  const int *state;        // {ring head, free blocks}
+  int *state_out;          // the same after the call, the rows in all, the requests refused
+  const int *owned;        // [n] blocks of each request
+  int *owned_out;
+  int *table;              // [n][width] block ids
+  int width;
+  int *row_start;          // [n + 1]
+  int *row_seq, *slots;    // [rows_cap]
+  int rows_cap;
+};
+cudaError_t launch_block_tables(const BlockTablesArgs &a, int sms, cudaStream_t s);
+
+// Rows of K then V (kv_heads * hd elements each, row stride `stride`) into their slots of the pool
+// (nslots = blocks * bs); slots outside the pool are skipped.
+cudaError_t launch_pack_slots(const void *x, int x_f16, long long stride, const int *slots,
+                              int rows, __half *pool, int nslots, int bs, int kv_heads, int hd,
+                              int sms, cudaStream_t s);
+
+struct AttendTreeArgs {
+  const void *q;
+  long long q_stride;    // elements between rows
+  void *o;
+  long long o_stride;
+  const __half *pool;
+  int blocks, bs;
+  const int *table;      // [n][width]
+  int width;
+  const int *row_start;  // [n + 1]; nullptr: request s has row s
+  const int *lens;       // [n]
+  const uint32_t *mask;  // [rows][words]; nullptr: no drafted positions
+  int words;
+  int rows, max_rows, max_len;
+  int heads, kv_heads, hd;
+  float scale;           // 1 / sqrt(hd)
+};
+cudaError_t launch_attend_tree(const AttendTreeArgs &a, int f16, int n, cudaStream_t s);
+
+struct ShapeArgs {
+  const void *logits;
+  void *out;               // nullptr: the edited logits are not wanted
+  long long ld, ld_out;
+  int rows, vocab, n;
+  const int *history, *hist_len;  // [n][max_hist], [n]
+  int max_hist;
+  const float *penalties;  // [n][3]: repetition, presence, frequency
+  const int *bias_ids;     // [n][max_bias]
+  const float *bias_vals;
+  const int *bias_len;
+  int max_bias;
+  const uint32_t *grammar; // [n_grammar][grammar_ld] words
+  int n_grammar, grammar_ld;
+  const int *grammar_of;   // [rows]
+  const int *row_seq;      // [rows]; nullptr: row r is request r
+  const int *row_start, *tokens;  // [n + 1], [rows]
+  const uint32_t *path;    // [rows][path_words]
+  int path_words;
+  int *picks;
+  float *logprobs;
+};
+cudaError_t launch_shape(const ShapeArgs &a, int f16, cudaStream_t s);
+
+struct TreeAcceptArgs {
+  const int *picks, *tokens;
+  const uint32_t *mask;    // [rows][words]
+  int words, rows;
+  const int *row_start;    // [n + 1]
+  int max_rows;
+  const int *lens, *table;
+  int width;
+  __half *pool;            // nullptr: nothing moves
+  long long layer_stride;  // elements
+  int blocks, bs, kv_heads, hd;
+  int *path, *count, *next, *new_lens;
+};
+cudaError_t launch_tree_accept(const TreeAcceptArgs &a, int n, int layers, cudaStream_t s);
+
 // ---- the log-mel frontend (frontend.cu) ----------------------------------------------------------
 
 // Device tables of the frontend, one image that the log-mel kernel copies into shared memory: the

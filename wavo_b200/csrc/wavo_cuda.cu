@@ -1533,6 +1533,258 @@ wavo_status wavo_attend(wavo_ctx *ctx, const float *q, const void *kv, float *pa
 
 // ---- graphs ------------------------------------------------------------------------------
 
+// ---- paged caches and drafted trees --------------------------------------------------------
+
+namespace {
+
+// The pool's shape: bs a power of two from 8 to 256, hd a multiple of 8 up to 128, slots in 31 bits.
+wavo_status check_pool(wavo_ctx *ctx, const char *who, const void *pool, uint32_t blocks,
+                       uint32_t bs, uint32_t kv_heads, uint32_t hd) {
+  if (bs < 8 || bs > 256 || (bs & (bs - 1)) || hd == 0 || hd % 8 || hd > 128 || kv_heads == 0 ||
+      kv_heads > 65535 || blocks == 0 || uint64_t(blocks) * bs > 0x7fffffffu)
+    return fail(ctx, WAVO_EINVAL, "%s: pool of %u blocks of %u positions, %u heads of %u", who,
+                blocks, bs, kv_heads, hd);
+  if (reinterpret_cast<uintptr_t>(pool) & 15u)
+    return fail(ctx, WAVO_EINVAL, "%s: the pool is not 16-byte aligned", who);
+  return WAVO_OK;
+}
+
+}  // namespace
+
+wavo_status wavo_block_tables(wavo_ctx *ctx, const int32_t *lens, const int32_t *adds, uint32_t n,
+                              uint32_t bs, int32_t *ring, uint32_t ring_cap, const int32_t *state,
+                              const int32_t *owned, int32_t *table, uint32_t width,
+                              int32_t *row_start, int32_t *row_seq, int32_t *slots,
+                              uint32_t rows_cap, int32_t *state_out, int32_t *owned_out) {
+  if (!ctx) return WAVO_EINVAL;
+  std::lock_guard<std::mutex> g(ctx->mu);
+  if (n == 0) return WAVO_OK;
+  if (!lens || !adds || !ring || !state || !owned || !table || !row_start || !state_out ||
+      !owned_out || (rows_cap && (!row_seq || !slots)))
+    return fail(ctx, WAVO_EINVAL, "block_tables: NULL buffer");
+  if (bs < 8 || bs > 256 || (bs & (bs - 1)) || ring_cap == 0 || ring_cap > 0x7fffffffu / bs ||
+      width == 0 || uint64_t(n) * width > 0x7fffffffu || uint64_t(width) * bs > 0x7fffffffu ||
+      rows_cap > 0x7fffffffu)
+    return fail(ctx, WAVO_EINVAL, "block_tables: %u requests, tables of %u blocks of %u positions, "
+                "ring of %u, %u rows", n, width, bs, ring_cap, rows_cap);
+  if (state == state_out || owned == owned_out)
+    return fail(ctx, WAVO_EINVAL, "block_tables: state_out and owned_out need buffers of their own");
+  cudaSetDevice(ctx->device);
+  const wv::BlockTablesArgs a = {lens,  adds,      int(n),  int(bs), ring,       int(ring_cap),
+                                 state, state_out, owned,   owned_out, table,    int(width),
+                                 row_start, row_seq, slots, int(rows_cap)};
+  CK(wv::launch_block_tables(a, ctx->sms, ctx->stream), "block_tables launch");
+  return WAVO_OK;
+}
+
+wavo_status wavo_pack_slots(wavo_ctx *ctx, const void *x, int x_dtype, uint32_t src,
+                            uint32_t stride, const int32_t *slots, uint32_t rows, void *pool,
+                            uint32_t blocks, uint32_t bs, uint32_t kv_heads, uint32_t hd) {
+  if (!ctx) return WAVO_EINVAL;
+  std::lock_guard<std::mutex> g(ctx->mu);
+  if (rows == 0) return WAVO_OK;
+  if (!x || !slots || !pool) return fail(ctx, WAVO_EINVAL, "pack_slots: NULL buffer");
+  if (x_dtype != WAVO_F32 && x_dtype != WAVO_F16)
+    return fail(ctx, WAVO_EINVAL, "pack_slots: dtype %d", x_dtype);
+  const wavo_status st = check_pool(ctx, "pack_slots", pool, blocks, bs, kv_heads, hd);
+  if (st != WAVO_OK) return st;
+  if (uint64_t(kv_heads) * hd > 0x3fffffffu || rows > 0x7fffffffu ||
+      (rows > 1 && stride < 2ull * kv_heads * hd))
+    return fail(ctx, WAVO_EINVAL, "pack_slots: %u rows of stride %u for K and V of %u heads of %u",
+                rows, stride, kv_heads, hd);
+  cudaSetDevice(ctx->device);
+  const int f16 = x_dtype == WAVO_F16;
+  const void *at = static_cast<const char *>(x) + size_t(src) * (f16 ? 2 : 4);
+  CK(wv::launch_pack_slots(at, f16, stride, slots, int(rows), static_cast<__half *>(pool),
+                           int(blocks * bs), int(bs), int(kv_heads), int(hd), ctx->sms,
+                           ctx->stream),
+     "pack_slots launch");
+  return WAVO_OK;
+}
+
+wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, int dtype,
+                             const void *pool, uint32_t blocks, uint32_t bs, const int32_t *table,
+                             uint32_t width, const int32_t *row_start, const int32_t *lens,
+                             uint32_t n, const uint32_t *mask, uint32_t mask_words, uint32_t rows,
+                             uint32_t max_rows, uint32_t max_len, void *o, uint64_t o_stride,
+                             uint32_t heads, uint32_t kv_heads, uint32_t hd) {
+  if (!ctx) return WAVO_EINVAL;
+  std::lock_guard<std::mutex> g(ctx->mu);
+  if (n == 0 || rows == 0 || max_rows == 0) return WAVO_OK;
+  if (!q || !pool || !table || !lens || !o)
+    return fail(ctx, WAVO_EINVAL, "attend_tree: NULL buffer");
+  if (dtype != WAVO_F32 && dtype != WAVO_F16)
+    return fail(ctx, WAVO_EINVAL, "attend_tree: dtype %d", dtype);
+  const wavo_status st = check_pool(ctx, "attend_tree", pool, blocks, bs, kv_heads, hd);
+  if (st != WAVO_OK) return st;
+  if (heads == 0 || heads > 65535 || heads % kv_heads)
+    return fail(ctx, WAVO_EINVAL, "attend_tree: %u heads over %u of the cache", heads, kv_heads);
+  if (q_stride == 0) q_stride = uint64_t(heads) * hd;
+  if (o_stride == 0) o_stride = uint64_t(heads) * hd;
+  if (q_stride < uint64_t(heads) * hd || o_stride < uint64_t(heads) * hd ||
+      (q_stride | o_stride) >> 31)
+    return fail(ctx, WAVO_EINVAL, "attend_tree: rows of %u heads of %u, strides %llu and %llu",
+                heads, hd, (unsigned long long)q_stride, (unsigned long long)o_stride);
+  if (width == 0 || uint64_t(n) * width > 0x7fffffffu || uint64_t(width) * bs > 0x7fffffffu ||
+      n > 65535 || rows > 0x7fffffffu || max_len > 0x7fffffffu)
+    return fail(ctx, WAVO_EINVAL, "attend_tree: %u requests, tables of %u blocks of %u positions, "
+                "%u rows", n, width, bs, rows);
+  if (mask && (mask_words == 0 || mask_words > 8 || max_rows > 32 * mask_words))
+    return fail(ctx, WAVO_EINVAL, "attend_tree: %u rows a request, %u mask words", max_rows,
+                mask_words);
+  if (!row_start && (max_rows > 1 || rows < n))
+    return fail(ctx, WAVO_EINVAL, "attend_tree: %u rows of %u requests without row_start", rows, n);
+  if (max_rows > rows) max_rows = rows;
+  cudaSetDevice(ctx->device);
+  wv::AttendTreeArgs a = {};
+  a.q = q;
+  a.q_stride = (long long)q_stride;
+  a.o = o;
+  a.o_stride = (long long)o_stride;
+  a.pool = static_cast<const __half *>(pool);
+  a.blocks = int(blocks);
+  a.bs = int(bs);
+  a.table = table;
+  a.width = int(width);
+  a.row_start = row_start;
+  a.lens = lens;
+  a.mask = mask;
+  a.words = mask ? int(mask_words) : 0;
+  a.rows = int(rows);
+  a.max_rows = int(max_rows);
+  a.max_len = int(max_len);
+  a.heads = int(heads);
+  a.kv_heads = int(kv_heads);
+  a.hd = int(hd);
+  a.scale = 1.0f / std::sqrt(float(hd));
+  CK(wv::launch_attend_tree(a, dtype == WAVO_F16, int(n), ctx->stream), "attend_tree launch");
+  return WAVO_OK;
+}
+
+size_t wavo_attend_tree_scratch(const wavo_ctx *, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t,
+                                uint32_t, uint32_t) {
+  return 0;
+}
+
+wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint64_t ld, void *out,
+                              uint64_t ld_out, uint32_t rows, const wavo_logit_rules *r,
+                              int32_t *picks, float *logprobs) {
+  if (!ctx) return WAVO_EINVAL;
+  std::lock_guard<std::mutex> g(ctx->mu);
+  if (rows == 0) return WAVO_OK;
+  if (!logits || !r) return fail(ctx, WAVO_EINVAL, "shape_logits: NULL buffer");
+  if (dtype != WAVO_F32 && dtype != WAVO_F16)
+    return fail(ctx, WAVO_EINVAL, "shape_logits: dtype %d", dtype);
+  if (ld == 0) ld = r->vocab;
+  if (ld_out == 0) ld_out = r->vocab;
+  if (r->vocab == 0 || r->vocab > 0x7fff0000u || ld < r->vocab || ld_out < r->vocab ||
+      (ld | ld_out) >> 31 || r->n == 0 || r->n > 0x7fffffffu || rows > 0x7fffffffu)
+    return fail(ctx, WAVO_EINVAL, "shape_logits: %u rows of %u tokens, strides %llu and %llu, %u "
+                "requests", rows, r->vocab, (unsigned long long)ld, (unsigned long long)ld_out, r->n);
+  if (out == logits && ld_out != ld)
+    return fail(ctx, WAVO_EINVAL, "shape_logits: in place with strides %llu and %llu",
+                (unsigned long long)ld, (unsigned long long)ld_out);
+  if (!r->row_seq && rows > r->n)
+    return fail(ctx, WAVO_EINVAL, "shape_logits: %u rows of %u requests without row_seq", rows,
+                r->n);
+  if ((r->history && (!r->hist_len || !r->max_hist)) ||
+      (r->path && (!r->path_words || !r->row_start || !r->tokens)) ||
+      (r->bias_ids && (!r->bias_vals || !r->bias_len || !r->max_bias)) ||
+      (r->grammar && (!r->grammar_of || !r->n_grammar)))
+    return fail(ctx, WAVO_EINVAL, "shape_logits: a rule without one of its buffers or sizes");
+  if ((r->history ? uint64_t(r->max_hist) : 0) + (r->path ? 32ull * r->path_words : 0) > 65535 ||
+      (r->bias_ids && r->max_bias > 65534))
+    return fail(ctx, WAVO_EINVAL, "shape_logits: %u tokens of history, %u path words, %u biases",
+                r->max_hist, r->path_words, r->max_bias);
+  if (r->grammar && (uint64_t(r->grammar_ld) * 32 < r->vocab || r->n_grammar > 0x7fffffffu))
+    return fail(ctx, WAVO_EINVAL, "shape_logits: %u grammar words for %u tokens", r->grammar_ld,
+                r->vocab);
+  cudaSetDevice(ctx->device);
+  wv::ShapeArgs a = {};
+  a.logits = logits;
+  a.out = out;
+  a.ld = (long long)ld;
+  a.ld_out = (long long)ld_out;
+  a.rows = int(rows);
+  a.vocab = int(r->vocab);
+  a.n = int(r->n);
+  a.history = r->history;
+  a.hist_len = r->hist_len;
+  a.max_hist = int(r->max_hist);
+  a.penalties = r->penalties;
+  a.bias_ids = r->bias_ids;
+  a.bias_vals = r->bias_vals;
+  a.bias_len = r->bias_len;
+  a.max_bias = int(r->max_bias);
+  a.grammar = r->grammar;
+  a.n_grammar = int(r->n_grammar);
+  a.grammar_ld = int(r->grammar_ld);
+  a.grammar_of = r->grammar_of;
+  a.row_seq = r->row_seq;
+  a.row_start = r->row_start;
+  a.tokens = r->tokens;
+  a.path = r->path;
+  a.path_words = int(r->path_words);
+  a.picks = picks;
+  a.logprobs = logprobs;
+  CK(wv::launch_shape(a, dtype == WAVO_F16, ctx->stream), "shape_logits launch");
+  return WAVO_OK;
+}
+
+wavo_status wavo_tree_accept(wavo_ctx *ctx, const int32_t *picks, const int32_t *tokens,
+                             const uint32_t *mask, uint32_t mask_words, uint32_t rows,
+                             const int32_t *row_start, uint32_t n, uint32_t max_rows,
+                             const int32_t *lens, const int32_t *table, uint32_t width, void *pool,
+                             uint32_t layers, uint64_t layer_stride, uint32_t blocks, uint32_t bs,
+                             uint32_t kv_heads, uint32_t hd, int32_t *path, int32_t *count,
+                             int32_t *next, int32_t *new_lens) {
+  if (!ctx) return WAVO_EINVAL;
+  std::lock_guard<std::mutex> g(ctx->mu);
+  if (n == 0) return WAVO_OK;
+  if (!picks || !tokens || !mask || !row_start || !lens || !path || !count || !next || !new_lens ||
+      (pool && !table))
+    return fail(ctx, WAVO_EINVAL, "tree_accept: NULL buffer");
+  if (mask_words == 0 || mask_words > 8 || max_rows == 0 || max_rows > 32 * mask_words ||
+      rows > 0x7fffffffu || n > 0x7fffffffu)
+    return fail(ctx, WAVO_EINVAL, "tree_accept: %u rows a request, %u mask words, %u rows, %u "
+                "requests", max_rows, mask_words, rows, n);
+  if (new_lens == lens)
+    return fail(ctx, WAVO_EINVAL, "tree_accept: new_lens needs a buffer of its own");
+  if (pool) {
+    const wavo_status st = check_pool(ctx, "tree_accept", pool, blocks, bs, kv_heads, hd);
+    if (st != WAVO_OK) return st;
+    if (width == 0 || uint64_t(width) * bs > 0x7fffffffu || layers == 0 || layers > 65535 ||
+        layer_stride % 8 ||
+        (layers > 1 && layer_stride < 2ull * blocks * bs * kv_heads * hd))
+      return fail(ctx, WAVO_EINVAL, "tree_accept: tables of %u blocks, %u layers %llu apart", width,
+                  layers, (unsigned long long)layer_stride);
+  }
+  cudaSetDevice(ctx->device);
+  wv::TreeAcceptArgs a = {};
+  a.picks = picks;
+  a.tokens = tokens;
+  a.mask = mask;
+  a.words = int(mask_words);
+  a.rows = int(rows);
+  a.row_start = row_start;
+  a.max_rows = int(max_rows);
+  a.lens = lens;
+  a.table = table;
+  a.width = int(width);
+  a.pool = static_cast<__half *>(pool);
+  a.layer_stride = (long long)layer_stride;
+  a.blocks = int(blocks);
+  a.bs = int(bs);
+  a.kv_heads = int(kv_heads);
+  a.hd = int(hd);
+  a.path = path;
+  a.count = count;
+  a.next = next;
+  a.new_lens = new_lens;
+  CK(wv::launch_tree_accept(a, int(n), pool ? int(layers) : 1, ctx->stream), "tree_accept launch");
+  return WAVO_OK;
+}
+
 wavo_status wavo_capture_begin(wavo_ctx *ctx) {
   if (!ctx) return WAVO_EINVAL;
   std::lock_guard<std::mutex> g(ctx->mu);

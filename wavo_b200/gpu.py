@@ -35,6 +35,28 @@ def _dtype(t: torch.Tensor) -> int:
     raise TypeError(f"unsupported buffer dtype {t.dtype} (float32 or float16)")
 
 
+def _contiguous_ptr(t: torch.Tensor) -> int:
+    if not t.is_contiguous():
+        raise ValueError("buffers are contiguous")
+    return _ptr(t)
+
+
+def _int32(*tensors) -> None:
+    """Contiguous int32 buffers (None: left out)."""
+    for t in tensors:
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
+            raise TypeError("contiguous int32 buffers")
+
+
+def _pool(pool: torch.Tensor, dims: int = 5) -> tuple[int, int, int, int]:
+    """blocks, kv_heads, bs, hd of a paged cache ([layers]) [blocks][2][kv_heads][bs][hd] f16."""
+    if pool.dtype is not torch.float16 or pool.dim() != dims or pool.shape[-4] != 2 or \
+            not pool.is_contiguous():
+        raise TypeError("a paged cache is contiguous f16 [blocks][2][kv_heads][bs][hd]")
+    blocks, _, kv_heads, bs, hd = pool.shape[-5:]
+    return blocks, kv_heads, bs, hd
+
+
 def pos_rows(t: int) -> int:
     """src/gpu/mod.rs:1060-1065."""
     return 2 * t + 15
@@ -391,6 +413,154 @@ class Pass:
         check(L.lib().wavo_attend_batch(self.ctx, _ptr(q), q_stride, _ptr(kv), kv_stride,
                                         _ptr(part), _ptr(o), o_stride, n, cols, heads, hd, batch),
               self.ctx)
+
+
+    def block_tables(self, lens: torch.Tensor, adds: torch.Tensor, bs: int, ring: torch.Tensor,
+                     state: torch.Tensor, owned: torch.Tensor, table: torch.Tensor,
+                     row_start: torch.Tensor, row_seq: torch.Tensor, slots: torch.Tensor,
+                     state_out: torch.Tensor, owned_out: torch.Tensor) -> None:
+        """Block tables and the slot map of a step's rows from the requests' lengths
+        (wavo_block_tables); int32 device tensors, table [n][width], row_start [n + 1], state [2],
+        state_out [4] (ring head, free blocks, rows, requests refused)."""
+        n = lens.numel()
+        _int32(lens, adds, ring, state, owned, table, row_start, row_seq, slots, state_out,
+               owned_out)
+        if table.shape[0] != n or adds.numel() != n or owned.numel() != n or \
+                owned_out.numel() != n or row_start.numel() != n + 1 or state.numel() < 2 or \
+                state_out.numel() < 4 or row_seq.numel() != slots.numel():
+            raise ValueError("block_tables: sizes differ")
+        check(L.lib().wavo_block_tables(
+            self.ctx, _ptr(lens), _ptr(adds), n, bs, _ptr(ring), ring.numel(), _ptr(state),
+            _ptr(owned), _ptr(table), table.shape[1], _ptr(row_start), _ptr(row_seq), _ptr(slots),
+            slots.numel(), _ptr(state_out), _ptr(owned_out)), self.ctx)
+
+    def pack_slots(self, x: torch.Tensor, src_stride: tuple[int, int], slots: torch.Tensor,
+                   pool: torch.Tensor) -> None:
+        """`pack` for a paged cache: one row of x (f32 or f16) for each of `slots` into pool
+        [blocks][2][kv_heads][bs][hd] (wavo_pack_slots)."""
+        blocks, kv_heads, bs, hd = _pool(pool)
+        _int32(slots)
+        src, stride = src_stride
+        rows = slots.numel()
+        if rows and src + (rows - 1) * stride + 2 * kv_heads * hd > x.numel():
+            raise ValueError("pack_slots: x has fewer rows")
+        check(L.lib().wavo_pack_slots(self.ctx, _ptr(x), _dtype(x), src, stride, _ptr(slots), rows,
+                                      _ptr(pool), blocks, bs, kv_heads, hd), self.ctx)
+
+    def attend_tree(self, q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor,
+                    lens: torch.Tensor, o: torch.Tensor, max_len: int,
+                    row_start: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                    max_rows: int = 1) -> None:
+        """Attention of rows q [rows][heads * hd] over a paged cache into o (wavo_attend_tree):
+        request s's rows row_start[s].. see its lens[s] positions and, with mask [rows][words], the
+        drafted positions behind them whose bits are set."""
+        blocks, kv_heads, bs, hd = _pool(pool)
+        _int32(table, lens, row_start, mask)
+        rows, wide = q.shape
+        n, width = table.shape
+        if q.stride(1) != 1 or o.stride(1) != 1 or o.shape != q.shape or o.dtype != q.dtype or \
+                wide % hd or lens.numel() != n or \
+                (row_start is not None and row_start.numel() != n + 1) or \
+                (mask is not None and mask.shape[0] < rows):
+            raise ValueError("attend_tree: sizes or types differ")
+        check(L.lib().wavo_attend_tree(
+            self.ctx, _ptr(q), q.stride(0), _dtype(q), _ptr(pool), blocks, bs, _ptr(table), width,
+            _ptr(row_start), _ptr(lens), n, _ptr(mask), 0 if mask is None else mask.shape[1], rows,
+            max_rows, max_len, _ptr(o), o.stride(0), wide // hd, kv_heads, hd), self.ctx)
+
+    def shape_logits(self, logits: torch.Tensor, rules: "LogitRules", picks: torch.Tensor | None,
+                     logprobs: torch.Tensor | None = None, out: torch.Tensor | None = None) -> None:
+        """The logits [rows][vocab] edited by the rules into out (None: not wanted; may be logits),
+        their first maximum and its log-softmax (wavo_shape_logits)."""
+        rows = logits.shape[0]
+        _int32(picks)
+        rules.check(rows)
+        if logits.stride(1) != 1 or logits.shape[1] < rules.c.vocab or \
+                (out is not None and (out.stride(1) != 1 or out.dtype != logits.dtype or
+                                      out.shape[0] < rows or out.shape[1] < rules.c.vocab)) or \
+                (picks is not None and picks.numel() < rows) or \
+                (logprobs is not None and (logprobs.numel() < rows or
+                                           logprobs.dtype != torch.float32)):
+            raise ValueError("shape_logits: sizes or types differ")
+        check(L.lib().wavo_shape_logits(
+            self.ctx, _ptr(logits), _dtype(logits), logits.stride(0), _ptr(out),
+            0 if out is None else out.stride(0), rows, ctypes.byref(rules.c), _ptr(picks),
+            _ptr(logprobs)), self.ctx)
+
+    def tree_accept(self, picks: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor,
+                    row_start: torch.Tensor, lens: torch.Tensor, table: torch.Tensor | None,
+                    pool: torch.Tensor | None, path: torch.Tensor, count: torch.Tensor,
+                    next_tokens: torch.Tensor, new_lens: torch.Tensor) -> None:
+        """The drafted path that the picks confirm, and its K and V moved together in pool
+        [layers][blocks][2][kv_heads][bs][hd] (None: nothing moves) (wavo_tree_accept)."""
+        n, max_rows = path.shape
+        _int32(picks, tokens, mask, row_start, lens, table, path, count, next_tokens, new_lens)
+        rows = tokens.numel()
+        layers = layer = blocks = kv_heads = bs = hd = width = 0
+        if pool is not None:
+            layers, layer = pool.shape[0], pool.stride(0)
+            blocks, kv_heads, bs, hd = _pool(pool, 6)
+            width = table.shape[1]
+        if mask.shape[0] != rows or picks.numel() < rows or row_start.numel() != n + 1 or \
+                lens.numel() != n or count.numel() != n or next_tokens.numel() != n or \
+                new_lens.numel() != n or (table is not None and table.shape[0] != n):
+            raise ValueError("tree_accept: sizes differ")
+        check(L.lib().wavo_tree_accept(
+            self.ctx, _ptr(picks), _ptr(tokens), _ptr(mask), mask.shape[1], rows, _ptr(row_start),
+            n, max_rows, _ptr(lens), _ptr(table), width, _ptr(pool), layers, layer, blocks, bs,
+            kv_heads, hd, _ptr(path), _ptr(count), _ptr(next_tokens), _ptr(new_lens)), self.ctx)
+
+
+class LogitRules:
+    """What `Pass.shape_logits` applies (wavo_logit_rules): made once over buffers whose contents
+    the decode loop rewrites. history = (tokens [n][max_hist], lengths [n]); tree = (row_seq [rows],
+    row_start [n + 1], tokens [rows], path [rows][words]); penalties [n][3] f32 (repetition,
+    presence, frequency); bias = (ids [n][most], values, counts [n]); grammar = (allowed-token bits
+    [sets][words], the set of each row [rows], -1 for none). Each part may be None; without a tree
+    row r is request r."""
+
+    def __init__(self, vocab: int, n: int | None = None, history=None, penalties=None, bias=None,
+                 grammar=None, tree=None):
+        self._keep = (history, penalties, bias, grammar, tree)
+        c = self.c = L.LogitRulesC()
+        sizes = [n] if n is not None else []
+        self._rows = []  # buffers with a value a row hold at least the call's rows
+        if history is not None:
+            _int32(*history)
+            sizes += [history[0].shape[0], history[1].numel()]
+            c.history, c.hist_len, c.max_hist = *map(_ptr, history), history[0].shape[1]
+        if penalties is not None:
+            if penalties.dtype != torch.float32 or penalties.shape[1] != 3:
+                raise ValueError("LogitRules: penalties are f32 [n][3]")
+            sizes.append(penalties.shape[0])
+            c.penalties = _contiguous_ptr(penalties)
+        if bias is not None:
+            ids, vals, count = bias
+            _int32(ids, count)
+            if vals.dtype != torch.float32 or vals.shape != ids.shape:
+                raise ValueError("LogitRules: bias values are f32, as many as ids")
+            sizes += [ids.shape[0], count.numel()]
+            c.bias_ids, c.bias_vals, c.bias_len = _ptr(ids), _contiguous_ptr(vals), _ptr(count)
+            c.max_bias = ids.shape[1]
+        if tree is not None:
+            row_seq, row_start, tokens, path = tree
+            _int32(*tree)
+            c.row_seq, c.row_start, c.tokens, c.path = map(_ptr, tree)
+            c.path_words = path.shape[1]
+            sizes.append(row_start.numel() - 1)
+            self._rows += [row_seq.numel(), tokens.numel(), path.shape[0]]
+        if grammar is not None:
+            _int32(*grammar)
+            c.grammar, c.grammar_of = map(_ptr, grammar)
+            c.n_grammar, c.grammar_ld = grammar[0].shape
+            self._rows.append(grammar[1].numel())
+        if len(set(sizes)) != 1:
+            raise ValueError(f"LogitRules: numbers of requests {sizes}")
+        c.vocab, c.n = vocab, sizes[0]
+
+    def check(self, rows: int) -> None:
+        if self._rows and min(self._rows) < rows:
+            raise ValueError("shape_logits: a rule has fewer rows than the logits")
 
 
 def partition_lpt(costs, parts: int) -> list[int]:
