@@ -224,8 +224,20 @@ struct AttendTreeArgs {
   int rows, max_rows, max_len;
   int heads, kv_heads, hd;
   float scale;           // 1 / sqrt(hd)
+  int splits, chunk;     // ranges of `chunk` positions, one CTA each
+  float *part;           // splits > 1: [rows][heads][splits][hd + 4] sums, maximum, sum of weights
+  int *err;              // device error word
 };
-cudaError_t launch_attend_tree(const AttendTreeArgs &a, int f16, int n, cudaStream_t s);
+// How a call is cut up: row_tiles CTAs of row_tile rows for each request and K and V head, each over
+// `splits` ranges of `chunk` positions.
+struct AttendTreePlan {
+  int row_tile, row_tiles, splits, chunk;
+};
+AttendTreePlan attend_tree_plan(int n, int max_rows, int max_len, int heads, int kv_heads, int sms);
+// map: the pool as a 4D f16 tensor {hd, bs, 2 kv_heads, blocks}, boxes {64, min(bs, 64), 1, 1},
+// 128-byte swizzle, zeros outside.
+cudaError_t launch_attend_tree(const CUtensorMap &map, const AttendTreeArgs &a,
+                               const AttendTreePlan &p, int f16, int n, cudaStream_t s);
 
 struct ShapeArgs {
   const void *logits;

@@ -3,87 +3,497 @@
 // Row i of a request sees its len cached positions and, with a mask, those of the rows drafted with
 // it whose bits its mask words hold (row j's K and V are at position len + j). o = softmax(q.k /
 // sqrt(hd)) v over what it sees, zeros where it sees nothing.
+//
+// One pass over K and V with the softmax's running maximum and sum: a CTA takes the rows of one K and V
+// head of one request (all its drafted rows and the heads that share it, MT at most) over a range
+// of positions, so that K and V are read once for them all. A producer warp loads 64 positions at a
+// time, page by page, through TMA boxes that follow the block table; four warps multiply.
+#include <algorithm>
+#include <type_traits>
+
 #include "kernels.cuh"
 #include "ptx.cuh"
 
 namespace wv {
 namespace {
 
-constexpr int TS_THREADS = 128;
+constexpr int TT_KEYS = 64;              // positions a tile
+constexpr int TT_WARPS = 4;              // multiplying warps
+constexpr int TT_THREADS = TT_WARPS * 32 + 32;
+constexpr uint32_t TT_HALF = TT_KEYS * 128;  // bytes of 64 positions x 64 elements
 
-// One CTA a (row, head, request): 128 keys a step, a key a thread for the scores, then an
-// element a thread for the values; the running maximum and sum as usual.
-template <typename T>
-__global__ void __launch_bounds__(TS_THREADS) attend_tree_kernel(const AttendTreeArgs a) {
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar,
+                                            int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+// c[16 x 8] += a[16 x 16] b[16 x 8], f16 in, f32 sums.
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                      uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Byte offset of 16-byte chunk `chunk` of tile row `row`: halves of 64 elements one after another.
+__device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t chunk) {
+  return (chunk >> 3) * TT_HALF + sw128_offset(row, chunk & 7u);
+}
+
+// hi + lo = (x, y) to 2^-22 of each.
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  hi = pack_half2(x, y);
+  const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&hi));
+  lo = pack_half2(x - f.x, y - f.y);
+}
+
+// The pair with zeros for infinities and NaN.
+__device__ __forceinline__ uint32_t finite2(uint32_t v) {
+  if ((v & 0x7c00u) == 0x7c00u) v &= 0xffff0000u;
+  if ((v & 0x7c000000u) == 0x7c000000u) v &= 0x0000ffffu;
+  return v;
+}
+
+// The multiplying warps alone.
+__device__ __forceinline__ void warps_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(TT_WARPS * 32) : "memory");
+}
+
+// HDP: head size padded to 64 or 128. MT: rows of a CTA; its warps take 16 each, and where that
+// leaves warps over, they share the tile's positions. WIDE: f32 rows, as two f16 parts each.
+template <int HDP, int MT, bool WIDE>
+struct TreeTile {
+  static constexpr int kWR = MT / 16, kWK = TT_WARPS / kWR;
+  static constexpr int kKeys = TT_KEYS / kWK;  // positions a warp takes of a tile
+  static constexpr uint32_t kStage = 2 * (HDP / 64) * TT_HALF;
+  static constexpr int kStages = HDP == 64 ? 4 : 3;
+  static constexpr size_t kSmem = kStages * kStage + 1024;
+};
+
+template <int HDP, int MT, bool WIDE>
+__global__ void __launch_bounds__(TT_THREADS)
+    attend_tree_kernel(const __grid_constant__ CUtensorMap map, const AttendTreeArgs a) {
+  using T = TreeTile<HDP, MT, WIDE>;
+  using E = typename std::conditional<WIDE, float, __half>::type;
+  constexpr int KS = HDP / 16, NT = T::kKeys / 8, ST = T::kStages;
+  extern __shared__ uint8_t raw[];
+  uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[ST], empty[ST];
+  __shared__ uint32_t info[ST];  // bit b: box b is in the pool; bit 31: every row sees all of it
+  __shared__ uint32_t abort_flag;
+  __shared__ float sh_m[T::kWK][MT], sh_l[T::kWK][MT];
+  const int tid = int(threadIdx.x), lane = tid & 31, w = int(warp_id());
+  const int split = int(blockIdx.x) % a.splits, r0 = int(blockIdx.x) / a.splits * MT;
+  const int kvh = int(blockIdx.y), s = int(blockIdx.z), group = a.heads / a.kv_heads;
+  const Abort ab{&abort_flag, a.err};
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], TT_WARPS);
+    }
+    abort_flag = 0u;
+    fence_mbar_init();
+    prefetch_tmap(&map);
+  }
   griddep_launch_dependents();
   griddep_wait();  // the previous kernel of the stream has completed (programmatic launch)
-  __shared__ float qs[128], ps[TS_THREADS], red[TS_THREADS / 32];
-  __shared__ long long at[TS_THREADS];
-  const int i = int(blockIdx.x), h = int(blockIdx.y), s = int(blockIdx.z);
-  const int tid = int(threadIdx.x), lane = tid & 31, w = tid >> 5;
+  __syncthreads();
+
   const int lo = a.row_start ? a.row_start[s] : s;
   const int t = min(a.row_start ? a.row_start[s + 1] - lo : 1, a.max_rows);
-  const int row = lo + i;
-  if (i >= t || row < 0 || row >= a.rows) return;
-  const T *q = static_cast<const T *>(a.q) + row * a.q_stride + h * a.hd;
-  if (tid < a.hd) qs[tid] = float(q[tid]);
-  const long long tile = (long long)a.bs * a.hd;
-  const int kvh = h / (a.heads / a.kv_heads);
-  const int *table = a.table + (long long)s * a.width;
+  const int rows = t * group;  // of this K and V head: token by token, the heads of each together
+  if (r0 >= rows || lo < 0) return;
   const int len = max(a.lens[s], 0);
   const int keys = int(min((long long)len + (a.mask ? t : 0), (long long)a.width * a.bs));
-  float m = -INFINITY, l = 0.0f, acc = 0.0f;
-  __syncthreads();
-  for (int j0 = 0; j0 < keys; j0 += TS_THREADS) {
-    const int j = j0 + tid;
-    float x = -INFINITY;
-    if (j < keys) {
-      const int d = j - len;
-      const bool seen = d < 0 || (d < 32 * a.words &&
-                                  ((a.mask[(long long)row * a.words + (d >> 5)] >> (d & 31)) & 1u));
-      const int b = table[j / a.bs];
-      if (seen && b >= 0 && b < a.blocks) {
-        const long long o = ((long long)b * 2 * a.kv_heads + kvh) * tile + (long long)(j % a.bs) * a.hd;
-        at[tid] = o + a.kv_heads * tile;
-        x = 0.0f;
-        for (int e = 0; e < a.hd; ++e) x = fmaf(qs[e], __half2float(a.pool[o + e]), x);
-        x *= a.scale;
+  const int k0 = split * a.chunk, k1 = min(keys, k0 + a.chunk);
+  const int n_tiles = k1 > k0 ? (k1 - k0 + TT_KEYS - 1) / TT_KEYS : 0;
+
+  if (w == TT_WARPS) {  // the producer
+    const int box = min(a.bs, TT_KEYS), boxes = TT_KEYS / box;
+    const int *table = a.table + (long long)s * a.width;
+    int i = 0;
+    for (; i < n_tiles; ++i) {
+      const int st = i % ST, pos = k0 + i * TT_KEYS + lane * box;
+      int b = -1;
+      if (lane < boxes && pos < keys) b = table[pos / a.bs];
+      const bool in = b >= 0 && b < a.blocks;
+      const uint32_t bits = __ballot_sync(0xffffffffu, in);
+      if (i >= ST && !mbar_wait_warp(&empty[st], ((i / ST) - 1) & 1, ab, kErrTimeoutProducer)) break;
+      if (lane == 0) {
+        const bool all = bits == (boxes == 32 ? ~0u : (1u << boxes) - 1u) &&
+                         k0 + (i + 1) * TT_KEYS <= min(len, keys);
+        info[st] = bits | (all ? 1u << 31 : 0u);
+        mbar_arrive_expect_tx(&full[st], T::kStage);
+      }
+      __syncwarp();
+      if (lane < boxes) {
+        // A position outside the pool reads as zeros: block `blocks` is past the tensor's end.
+        uint8_t *to = tiles + st * T::kStage + lane * box * 128;
+        const int z = in ? b : a.blocks;
+#pragma unroll
+        for (int h = 0; h < HDP / 64; ++h) {
+          tma_load_4d(to + h * TT_HALF, &map, &full[st], 64 * h, pos % a.bs, kvh, z);
+          tma_load_4d(to + (HDP / 64 + h) * TT_HALF, &map, &full[st], 64 * h, pos % a.bs,
+                      a.kv_heads + kvh, z);
+        }
       }
     }
-    float mx = x;
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (lane == 0) red[w] = mx;
-    __syncthreads();
-    for (int k = 0; k < TS_THREADS / 32; ++k) mx = fmaxf(mx, red[k]);
-    const float m1 = fmaxf(m, mx);
-    if (m1 != -INFINITY) {
-      const float c = __expf(m - m1);
-      ps[tid] = x == -INFINITY ? 0.0f : __expf(x - m1);
-      l *= c;
-      acc *= c;
-      m = m1;
-    } else {
-      ps[tid] = 0.0f;
-    }
-    __syncthreads();
-    for (int k = 0; k < min(TS_THREADS, keys - j0); ++k)
-      if (ps[k] != 0.0f) {
-        l += ps[k];
-        if (tid < a.hd) acc = fmaf(ps[k], __half2float(a.pool[at[k] + tid]), acc);
-      }
-    __syncthreads();
+    // The shared memory stays until the last loads have landed, also where a wait gave up.
+    for (int j = max(i - ST, 0); j < i; ++j)
+      for (int k = 0; k < 2000 && !mbar_try_wait_sleep(&full[j % ST], (j / ST) & 1, 100000u); ++k) {}
+    return;
   }
-  if (tid < a.hd)
-    (static_cast<T *>(a.o) + row * a.o_stride + h * a.hd)[tid] = T(l != 0.0f ? acc / l : 0.0f);
+
+  const int wr = w % T::kWR, wk = w / T::kWR;
+  const int g = lane >> 2, c2 = (lane & 3) * 2;
+  // This thread's rows r and r + 8 of the CTA's.
+  int row[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = r0 + wr * 16 + g + 8 * u, i = r / group;
+    row[u] = r < rows && lo + i < a.rows ? lo + i : -1;
+  }
+  uint32_t qh[KS][4], ql[WIDE ? KS : 1][4];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int u = x & 1, c = 16 * ks + c2 + 8 * (x >> 1);
+      const int head = kvh * group + (r0 + wr * 16 + g + 8 * u) % group;
+      E v[2] = {E(0.0f), E(0.0f)};
+      if (row[u] >= 0 && c < a.hd) {
+        const E *p = static_cast<const E *>(a.q) + row[u] * a.q_stride + head * a.hd + c;
+        v[0] = p[0];
+        v[1] = p[1];
+      }
+      if constexpr (WIDE) split2(v[0], v[1], qh[ks][x], ql[ks][x]);
+      else qh[ks][x] = uint32_t(__half_as_ushort(v[0])) | uint32_t(__half_as_ushort(v[1])) << 16;
+    }
+  float acc[2 * KS][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  const float scale = a.scale * 1.4426950408889634f;  // exponentials of base 2
+  bool ok = true;
+  for (int i = 0; i < n_tiles; ++i) {
+    const int st = i % ST;
+    ok = mbar_wait_warp(&full[st], (i / ST) & 1, ab, kErrTimeoutConsumer);
+    if (!ok) break;
+    const uint32_t kb = smem_u32(tiles + st * T::kStage), vb = kb + (HDP / 64) * TT_HALF;
+    const uint32_t bits = info[st];
+    const int first = wk * T::kKeys;  // the warp's first position in the tile
+    const int p0 = k0 + i * TT_KEYS + first;
+    float sc[NT][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int n = 0; n < NT / 2; ++n) {
+        uint32_t b[4];
+        ldsm4(b, kb + tile_at(first + n * 16 + (lane >> 4) * 8 + (lane & 7),
+                              2 * ks + ((lane >> 3) & 1)));
+        mma16(sc[2 * n], qh[ks], b[0], b[1]);
+        mma16(sc[2 * n + 1], qh[ks], b[2], b[3]);
+        if constexpr (WIDE) {
+          mma16(sc[2 * n], ql[ks], b[0], b[1]);
+          mma16(sc[2 * n + 1], ql[ks], b[2], b[3]);
+        }
+      }
+    bool odd = false;  // a V row that some rows do not see holds an infinity or NaN
+    if (!(bits >> 31)) {
+      // Positions past the end, outside the pool, or drafted off a row's path.
+      const int box = min(a.bs, TT_KEYS);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int j = first + 8 * n + c2 + (x & 1), p = k0 + i * TT_KEYS + j, d = p - len;
+          bool see = p < k1 && ((bits >> (j / box)) & 1u);
+          if (see && d >= 0)
+            see = row[x >> 1] >= 0 && d < 32 * a.words &&
+                  ((a.mask[(long long)row[x >> 1] * a.words + (d >> 5)] >> (d & 31)) & 1u);
+          if (!see) sc[n][x] = -INFINITY;
+        }
+      // What lies in a page past the end is nobody's: zeros in V (0 times NaN is not 0).
+      if (p0 + T::kKeys > k1) {
+        const int from = max(k1 - p0, 0);
+        for (int e = lane; e < (T::kKeys - from) * (HDP / 8); e += 32) {
+          const uint32_t at = vb + tile_at(first + from + e / (HDP / 8), e % (HDP / 8));
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+        }
+        __syncwarp();
+      }
+      if (p0 + T::kKeys > len) {
+        bool bad = false;
+        for (int e = lane; e < T::kKeys * (HDP / 8); e += 32) {
+          uint32_t v[4];
+          const uint32_t at = vb + tile_at(first + e / (HDP / 8), e % (HDP / 8));
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                       : "r"(at)
+                       : "memory");
+#pragma unroll
+          for (int k = 0; k < 4; ++k) bad = bad || finite2(v[k]) != v[k];
+        }
+        odd = __any_sync(0xffffffffu, bad);
+      }
+    }
+    // The running maximum and sum, two rows a thread (four threads a row).
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float mx = m[u];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * u], sc[n][2 * u + 1]) * scale);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float base = mx == -INFINITY ? 0.0f : mx;
+      const float carry = ex2(m[u] - base);
+      m[u] = mx;
+      float sum = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 2 * u; x < 2 * u + 2; ++x) {
+          sc[n][x] = ex2(fmaf(sc[n][x], scale, -base));
+          sum += sc[n][x];
+        }
+      l[u] = fmaf(l[u], carry, sum);
+      if (__any_sync(0xffffffffu, carry != 1.0f))
+#pragma unroll
+        for (int n = 0; n < 2 * KS; ++n) {
+          acc[n][2 * u] *= carry;
+          acc[n][2 * u + 1] *= carry;
+        }
+    }
+    const auto values = [&](auto clean) {
+#pragma unroll
+      for (int kk = 0; kk < NT / 2; ++kk) {
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float p = sc[2 * kk + (x >> 1)][2 * (x & 1)], q = sc[2 * kk + (x >> 1)][2 * (x & 1) + 1];
+          if constexpr (WIDE) split2(p, q, ph[x], pl[x]);
+          else ph[x] = pack_half2(p, q);
+        }
+#pragma unroll
+        for (int n = 0; n < KS; ++n) {
+          uint32_t b[4];
+          ldsm4_t(b, vb + tile_at(first + kk * 16 + (lane & 15), 2 * n + (lane >> 4)));
+          if constexpr (decltype(clean)::value)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) b[x] = finite2(b[x]);
+          mma16(acc[2 * n], ph, b[0], b[1]);
+          mma16(acc[2 * n + 1], ph, b[2], b[3]);
+          if constexpr (WIDE) {
+            mma16(acc[2 * n], pl, b[0], b[1]);
+            mma16(acc[2 * n + 1], pl, b[2], b[3]);
+          }
+        }
+      }
+    };
+    if (!odd) {
+      values(std::false_type());
+    } else {
+      // Infinities and NaN in V go one by one to the rows that see them, and the products get
+      // zeros in their place (0 times infinity is not 0).
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+          const int from = (lane & ~3) | (j >> 1);
+          float p[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float e = __shfl_sync(0xffffffffu, sc[n][2 * u], from);
+            const float f = __shfl_sync(0xffffffffu, sc[n][2 * u + 1], from);
+            p[u] = (j & 1) ? f : e;
+          }
+#pragma unroll
+          for (int c = 0; c < 2 * KS; ++c) {
+            uint32_t v;
+            asm volatile("ld.shared.b32 %0, [%1];"
+                         : "=r"(v)
+                         : "r"(vb + tile_at(first + 8 * n + j, c) + 2 * c2)
+                         : "memory");
+            const uint32_t rest = v ^ finite2(v);
+            if (rest == 0u) continue;
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&rest));
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              if (p[u] != 0.0f) {
+                acc[c][2 * u] = fmaf(p[u], f.x, acc[c][2 * u]);
+                acc[c][2 * u + 1] = fmaf(p[u], f.y, acc[c][2 * u + 1]);
+              }
+          }
+        }
+      values(std::true_type());
+    }
+    if (!(bits >> 31)) fence_proxy_async_smem();  // the zeros, before a later load
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[st]);
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+  }
+
+  // The warps' shares of the positions meet in shared memory, over the tiles.
+  float *sum = reinterpret_cast<float *>(tiles);  // [kWK][MT][HDP]
+  warps_sync();
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = wr * 16 + g + 8 * u;
+    if ((lane & 3) == 0) {
+      sh_m[wk][r] = m[u];
+      sh_l[wk][r] = l[u];
+    }
+#pragma unroll
+    for (int n = 0; n < 2 * KS; ++n)
+      *reinterpret_cast<float2 *>(sum + (wk * MT + r) * HDP + 8 * n + c2) =
+          make_float2(acc[n][2 * u], acc[n][2 * u + 1]);
+  }
+  warps_sync();
+  if (abort_flag) return;  // a wait gave up: the outputs are left as they are
+  const int quads = a.hd / 4;
+  for (int e = tid; e < MT * quads; e += TT_WARPS * 32) {
+    const int r = e / quads, c = (e - r * quads) * 4, rr = r0 + r;
+    if (rr >= rows) break;
+    const int q = lo + rr / group, head = kvh * group + rr % group;
+    if (q >= a.rows) break;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < T::kWK; ++k) top = fmaxf(top, sh_m[k][r]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f, o[4] = {};
+#pragma unroll
+    for (int k = 0; k < T::kWK; ++k) {
+      const float f = ex2(sh_m[k][r] - base);
+      const float4 v = *reinterpret_cast<const float4 *>(sum + (k * MT + r) * HDP + c);
+      total = fmaf(f, sh_l[k][r], total);
+      o[0] = fmaf(f, v.x, o[0]);
+      o[1] = fmaf(f, v.y, o[1]);
+      o[2] = fmaf(f, v.z, o[2]);
+      o[3] = fmaf(f, v.w, o[3]);
+    }
+    if (a.splits == 1) {
+      const float inv = total != 0.0f ? 1.0f / total : 0.0f;
+      E *to = static_cast<E *>(a.o) + q * a.o_stride + (long long)head * a.hd + c;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) to[x] = E(o[x] * inv);
+    } else {
+      float *to = a.part + (((long long)q * a.heads + head) * a.splits + split) * (a.hd + 4);
+      *reinterpret_cast<float4 *>(to + c) = make_float4(o[0], o[1], o[2], o[3]);
+      if (c == 0) *reinterpret_cast<float2 *>(to + a.hd) = make_float2(top, total);
+    }
+  }
+}
+
+// The ranges of a row joined: a CTA a (drafted row, request), four elements a thread.
+template <typename E>
+__global__ void __launch_bounds__(128) attend_tree_join_kernel(const AttendTreeArgs a) {
+  griddep_launch_dependents();
+  griddep_wait();  // the previous kernel of the stream has completed (programmatic launch)
+  const int i = int(blockIdx.x), s = int(blockIdx.z);
+  const int lo = a.row_start ? a.row_start[s] : s;
+  const int t = min(a.row_start ? a.row_start[s + 1] - lo : 1, a.max_rows), q = lo + i;
+  if (i >= t || lo < 0 || q >= a.rows) return;
+  const int quads = a.hd / 4;
+  for (int e = int(blockIdx.y * blockDim.x + threadIdx.x); e < a.heads * quads;
+       e += int(gridDim.y * blockDim.x)) {
+    const int head = e / quads, c = (e - head * quads) * 4;
+    const float *from = a.part + ((long long)q * a.heads + head) * a.splits * (a.hd + 4);
+    float top = -INFINITY;
+    for (int k = 0; k < a.splits; ++k) top = fmaxf(top, from[k * (a.hd + 4) + a.hd]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f, o[4] = {};
+    for (int k = 0; k < a.splits; ++k) {
+      const float2 ml = *reinterpret_cast<const float2 *>(from + k * (a.hd + 4) + a.hd);
+      const float4 v = *reinterpret_cast<const float4 *>(from + k * (a.hd + 4) + c);
+      const float f = ex2(ml.x - base);
+      total = fmaf(f, ml.y, total);
+      o[0] = fmaf(f, v.x, o[0]);
+      o[1] = fmaf(f, v.y, o[1]);
+      o[2] = fmaf(f, v.z, o[2]);
+      o[3] = fmaf(f, v.w, o[3]);
+    }
+    const float inv = total != 0.0f ? 1.0f / total : 0.0f;
+    E *to = static_cast<E *>(a.o) + q * a.o_stride + (long long)head * a.hd + c;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) to[x] = E(o[x] * inv);
+  }
+}
+
+template <int HDP, int MT, bool WIDE>
+cudaError_t launch_tile(const CUtensorMap &map, const AttendTreeArgs &a, int row_tiles, int n,
+                        cudaStream_t s) {
+  auto *kernel = attend_tree_kernel<HDP, MT, WIDE>;
+  constexpr size_t smem = TreeTile<HDP, MT, WIDE>::kSmem;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !configured[dev]) {
+    cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) configured[dev] = true;
+  }
+  return launch_pdl(kernel, dim3(a.splits * row_tiles, a.kv_heads, n), dim3(TT_THREADS), smem, s,
+                    map, a);
+}
+
+template <int HDP, bool WIDE>
+cudaError_t launch_rows(const CUtensorMap &map, const AttendTreeArgs &a, const AttendTreePlan &p,
+                        int n, cudaStream_t s) {
+  return p.row_tile == 16   ? launch_tile<HDP, 16, WIDE>(map, a, p.row_tiles, n, s)
+         : p.row_tile == 32 ? launch_tile<HDP, 32, WIDE>(map, a, p.row_tiles, n, s)
+                            : launch_tile<HDP, 64, WIDE>(map, a, p.row_tiles, n, s);
 }
 
 }  // namespace
 
-cudaError_t launch_attend_tree(const AttendTreeArgs &a, int f16, int n, cudaStream_t s) {
+AttendTreePlan attend_tree_plan(int n, int max_rows, int max_len, int heads, int kv_heads, int sms) {
+  AttendTreePlan p;
+  const long long rows = (long long)max_rows * (heads / kv_heads);
+  p.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  p.row_tiles = int((rows + p.row_tile - 1) / p.row_tile);
+  const long long ctas = (long long)n * kv_heads * p.row_tiles;
+  // Ranges of 256 positions at least, as many as fill the SMs four times.
+  const long long want = (4ll * sms + ctas - 1) / ctas;
+  const long long most = std::max<long long>(1, (max_len + 255) / 256);
+  p.splits = int(std::min<long long>(std::min(want, most), 128));
+  p.chunk = int(((long long)max_len + p.splits - 1) / p.splits);
+  p.chunk = std::max((p.chunk + TT_KEYS - 1) / TT_KEYS, 1) * TT_KEYS;
+  p.splits = std::max((max_len + p.chunk - 1) / p.chunk, 1);
+  return p;
+}
+
+cudaError_t launch_attend_tree(const CUtensorMap &map, const AttendTreeArgs &a,
+                               const AttendTreePlan &p, int f16, int n, cudaStream_t s) {
   if (n <= 0 || a.max_rows <= 0) return cudaSuccess;
-  const dim3 grid(a.max_rows, a.heads, n);
-  if (f16) return launch_pdl(attend_tree_kernel<__half>, grid, dim3(TS_THREADS), 0, s, a);
-  return launch_pdl(attend_tree_kernel<float>, grid, dim3(TS_THREADS), 0, s, a);
+  cudaError_t e;
+  if (a.hd <= 64)
+    e = f16 ? launch_rows<64, false>(map, a, p, n, s) : launch_rows<64, true>(map, a, p, n, s);
+  else
+    e = f16 ? launch_rows<128, false>(map, a, p, n, s) : launch_rows<128, true>(map, a, p, n, s);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  const dim3 grid(a.max_rows, std::min(8, (a.heads * a.hd / 4 + 127) / 128), n);
+  return f16 ? launch_pdl(attend_tree_join_kernel<__half>, grid, dim3(128), 0, s, a)
+             : launch_pdl(attend_tree_join_kernel<float>, grid, dim3(128), 0, s, a);
 }
 
 }  // namespace wv

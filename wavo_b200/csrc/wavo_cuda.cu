@@ -1537,6 +1537,21 @@ wavo_status wavo_attend(wavo_ctx *ctx, const float *q, const void *kv, float *pa
 
 namespace {
 
+// A paged cache as {hd, bs, 2 kv_heads, blocks} of f16, boxes of 64 elements x min(bs, 64) positions
+// of one head, 128-byte swizzle, zeros outside (past hd, and in block `blocks`).
+bool make_map_pool(CUtensorMap *m, const void *pool, uint64_t blocks, uint64_t bs,
+                   uint64_t kv_heads, uint64_t hd) {
+  EncodeTiled enc = encoder();
+  if (!enc) return false;
+  cuuint64_t dims[4] = {hd, bs, 2 * kv_heads, blocks};
+  cuuint64_t strides[3] = {hd * 2, bs * hd * 2, 2 * kv_heads * bs * hd * 2};
+  cuuint32_t box[4] = {64, cuuint32_t(std::min<uint64_t>(bs, 64)), 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(pool), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // The pool's shape: bs a power of two from 8 to 256, hd a multiple of 8 up to 128, slots in 31 bits.
 wavo_status check_pool(wavo_ctx *ctx, const char *who, const void *pool, uint32_t blocks,
                        uint32_t bs, uint32_t kv_heads, uint32_t hd) {
@@ -1657,13 +1672,36 @@ wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, in
   a.kv_heads = int(kv_heads);
   a.hd = int(hd);
   a.scale = 1.0f / std::sqrt(float(hd));
-  CK(wv::launch_attend_tree(a, dtype == WAVO_F16, int(n), ctx->stream), "attend_tree launch");
+  // Positions past the tables' end are nobody's.
+  const uint64_t reach = std::min<uint64_t>(max_len, uint64_t(width) * bs);
+  const wv::AttendTreePlan plan = wv::attend_tree_plan(int(n), int(max_rows), int(reach),
+                                                       int(heads), int(kv_heads), ctx->sms);
+  a.splits = plan.splits;
+  a.chunk = plan.chunk;
+  a.err = ctx->dev_err;
+  if (plan.splits > 1) {
+    void *ws = nullptr;
+    const wavo_status got = workspace(
+        ctx, size_t(rows) * heads * plan.splits * (hd + 4) * sizeof(float), &ws);
+    if (got != WAVO_OK) return got;
+    a.part = static_cast<float *>(ws);
+  }
+  CUtensorMap map;
+  if (!make_map_pool(&map, pool, blocks, bs, kv_heads, hd))
+    return fail(ctx, WAVO_ECUDA, "attend_tree: tensor map");
+  CK(wv::launch_attend_tree(map, a, plan, dtype == WAVO_F16, int(n), ctx->stream),
+     "attend_tree launch");
   return WAVO_OK;
 }
 
-size_t wavo_attend_tree_scratch(const wavo_ctx *, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t,
-                                uint32_t, uint32_t) {
-  return 0;
+size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t n, uint32_t rows, uint32_t max_rows,
+                                uint32_t max_len, uint32_t heads, uint32_t kv_heads, uint32_t hd) {
+  if (!ctx || !n || !rows || !max_rows || !kv_heads || heads < kv_heads || max_len > 0x7fffffffu)
+    return 0;
+  const wv::AttendTreePlan p =
+      wv::attend_tree_plan(int(n), int(std::min(max_rows, rows)), int(max_len), int(heads),
+                           int(kv_heads), ctx->sms);
+  return p.splits > 1 ? size_t(rows) * heads * p.splits * (hd + 4) * sizeof(float) : 0;
 }
 
 wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint64_t ld, void *out,
