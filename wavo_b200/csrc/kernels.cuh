@@ -224,20 +224,19 @@ struct AttendTreeArgs {
   int rows, max_rows, max_len;
   int heads, kv_heads, hd;
   float scale;           // 1 / sqrt(hd)
-  int splits, chunk;     // ranges of `chunk` positions, one CTA each
-  float *part;           // splits > 1: [rows][heads][splits][hd + 4] sums, maximum, sum of weights
+  int n;                 // requests
+  float *part;           // parts of items that span several runs (attend_tree_part_bytes)
+  int *count;            // parts written of each, kTreeRunsPerSm a SM, 0 between launches
   int *err;              // device error word
 };
-// How a call is cut up: row_tiles CTAs of row_tile rows for each request and K and V head, each over
-// `splits` ranges of `chunk` positions.
-struct AttendTreePlan {
-  int row_tile, row_tiles, splits, chunk;
-};
-AttendTreePlan attend_tree_plan(int n, int max_rows, int max_len, int heads, int kv_heads, int sms);
-// map: the pool as a 4D f16 tensor {hd, bs, 2 kv_heads, blocks}, boxes {64, min(bs, 64), 1, 1},
+constexpr int kTreeRunsPerSm = 2;
+// Rows of an item: the rows of a request that read one K and V head, in steps that the kernel has.
+int attend_tree_rows(int max_rows, int heads, int kv_heads, int f16);
+size_t attend_tree_part_bytes(int max_rows, int heads, int kv_heads, int hd, int f16, int sms);
+// map: the pool as a 4D f16 tensor {hd, bs, 2 kv_heads, blocks}, boxes {64, min(bs, 128), 1, 1},
 // 128-byte swizzle, zeros outside.
-cudaError_t launch_attend_tree(const CUtensorMap &map, const AttendTreeArgs &a,
-                               const AttendTreePlan &p, int f16, int n, cudaStream_t s);
+cudaError_t launch_attend_tree(const CUtensorMap &map, const AttendTreeArgs &a, int f16, int sms,
+                               cudaStream_t s);
 
 struct ShapeArgs {
   const void *logits;

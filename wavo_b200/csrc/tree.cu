@@ -4,10 +4,21 @@
 // it whose bits its mask words hold (row j's K and V are at position len + j). o = softmax(q.k /
 // sqrt(hd)) v over what it sees, zeros where it sees nothing.
 //
-// One pass over K and V with the softmax's running maximum and sum: a CTA takes the rows of one K and V
-// head of one request (all its drafted rows and the heads that share it, MT at most) over a range
-// of positions, so that K and V are read once for them all. A producer warp loads 64 positions at a
-// time, page by page, through TMA boxes that follow the block table; four warps multiply.
+// One pass over K and V with a running softmax. An item is one K and V head of one request with all
+// the rows that read it (its drafted rows and the heads that share it, NR at most), so that K and V
+// are read once for them all. The rows are few and the positions many, so the products are turned:
+// 128 positions are the UMMA's M and the rows its N,
+//   S^T [128 x NR] = K [128 x hd] . Q^T,   O^T [hd x NR] += V^T [hd x 128] . P^T,
+// and a padded row costs N columns in steps of 16 where it would cost 128 lanes. A thread of the
+// softmax has one position and all the rows (or half of them): no row is reduced over lanes but where
+// its reference value has to rise. That is 8 (base 2) above it, at which a probability is still 256 in
+// f16, so it happens at an item's first tile and seldom after; a vote a tile asks.
+//
+// The items' tiles of 128 positions lie one after another and are cut into equal runs, one a CTA, as
+// many CTAs as are resident: ragged lengths, few long requests and many short ones fill the GPU alike,
+// and the loads run ahead across the items of a run. A run that ends inside an item leaves its
+// part in global memory; whichever CTA finishes an item's last part joins them, in the order
+// of the runs.
 #include <algorithm>
 #include <type_traits>
 
@@ -17,10 +28,11 @@
 namespace wv {
 namespace {
 
-constexpr int TT_KEYS = 64;              // positions a tile
-constexpr int TT_WARPS = 4;              // multiplying warps
-constexpr int TT_THREADS = TT_WARPS * 32 + 32;
-constexpr uint32_t TT_HALF = TT_KEYS * 128;  // bytes of 64 positions x 64 elements
+constexpr int TT_KEYS = 128;                  // positions a tile
+constexpr uint32_t TT_HALF = TT_KEYS * 128;   // bytes of 128 positions x 64 elements
+constexpr float TT_RISE = 8.0f;
+constexpr int TT_PIECES = 3;                  // items in flight: loaded, multiplied, written
+constexpr int TT_WHOLE = 4;                   // items of up to this many tiles stay in one run
 
 __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar,
                                             int x, int y, int z, int w) {
@@ -29,33 +41,6 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, u
       "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
-}
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(at)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(at)
-               : "memory");
-}
-// c[16 x 8] += a[16 x 16] b[16 x 8], f16 in, f32 sums.
-__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                      uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Byte offset of 16-byte chunk `chunk` of tile row `row`: halves of 64 elements one after another.
-__device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t chunk) {
-  return (chunk >> 3) * TT_HALF + sw128_offset(row, chunk & 7u);
 }
 
 // hi + lo = (x, y) to 2^-22 of each.
@@ -72,377 +57,772 @@ __device__ __forceinline__ uint32_t finite2(uint32_t v) {
   return v;
 }
 
-// The multiplying warps alone.
-__device__ __forceinline__ void warps_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(TT_WARPS * 32) : "memory");
+// v[k] of 32 lanes reduced for each k: lane k gets the result of v[k] (31 shuffles for 32 values; the
+// halves that a lane gives away it reads from its partner).
+template <bool MAX, int N>
+__device__ __forceinline__ float lanes_reduce(float (&v)[N]) {
+  const int lane = int(threadIdx.x) & 31;
+#pragma unroll
+  for (int h = 16; h > 0; h >>= 1) {
+    const bool up = (lane & h) != 0;
+#pragma unroll
+    for (int k = 0; k < h; ++k) {
+      const float give = up ? v[k] : v[k + h], keep = up ? v[k + h] : v[k];
+      const float got = __shfl_xor_sync(0xffffffffu, give, h);
+      v[k] = MAX ? fmaxf(keep, got) : keep + got;
+    }
+  }
+  return v[0];
 }
 
-// HDP: head size padded to 64 or 128. MT: rows of a CTA; its warps take 16 each, and where that
-// leaves warps over, they share the tile's positions. WIDE: f32 rows, as two f16 parts each.
-template <int HDP, int MT, bool WIDE>
+// HDP: head size padded to 64 or 128. NR: rows of an item. WIDE: f32 rows, as two f16 parts each.
+template <int HDP, int NR, bool WIDE>
 struct TreeTile {
-  static constexpr int kWR = MT / 16, kWK = TT_WARPS / kWR;
-  static constexpr int kKeys = TT_KEYS / kWK;  // positions a warp takes of a tile
-  static constexpr uint32_t kStage = 2 * (HDP / 64) * TT_HALF;
-  static constexpr int kStages = HDP == 64 ? 4 : 3;
-  static constexpr size_t kSmem = kStages * kStage + 1024;
+  static constexpr int kParts = WIDE ? 2 : 1;
+  static constexpr uint32_t kSlot = (HDP / 64) * TT_HALF;           // a tile of K or of V
+  static constexpr uint32_t kQ = (HDP / 64) * NR * 128;             // Q, one part
+  static constexpr uint32_t kP = (NR + 63) / 64 * TT_HALF;          // P, one part
+  // Up to 32 rows of heads of 64, two CTAs share an SM (113 KB of shared memory each); else one.
+  static constexpr int kCtas = HDP == 64 && NR <= 32 ? 2 : 1;
+  static constexpr int kPBufs = kCtas * kParts * kP >= 2 * TT_HALF ? 1 : 2;
+  static constexpr int kQBufs = kParts * kQ > 16384 ? 1 : 2;
+  static constexpr int kRing = HDP == 128 ? (kParts * NR >= 128 ? 3 : 4) : kCtas == 2 ? 4 : 8;
+  // Softmax warps: a group of four holds the 128 positions; two groups halve the rows.
+  static constexpr int kGroups = NR <= 32 ? 1 : 2;
+  static constexpr int kRows = NR / kGroups;                        // rows a thread holds
+  static constexpr int kSoft = 128 * kGroups;
+  static constexpr int kThreads = kSoft + 96;                       // and loads, UMMAs, rows
+  static constexpr uint32_t kOffQ = kRing * kSlot;
+  static constexpr uint32_t kOffP = kOffQ + kQBufs * kParts * kQ;
+  static constexpr uint32_t kOffBar = kOffP + kPBufs * kParts * kP;
+  static constexpr uint32_t kCols = NR == 16 ? 64 : NR == 32 ? 128 : NR == 64 ? 256 : 512;
 };
 
-template <int HDP, int MT, bool WIDE>
-__global__ void __launch_bounds__(TT_THREADS)
+// A run's share of an item.
+struct TreePiece {
+  int s, kvh, r0, here;     // request, K and V head, first row, rows
+  int lo, rows, len, keys;  // the request's first row, its drafted rows, positions without and with them
+  int tile0, tiles;         // tiles of the item
+  int slot;                 // where a partial result goes; -1: the item is whole
+  int first, parts;         // the run that the item begins in, the runs that it takes
+};
+
+template <int NR>
+struct TreeRows {
+  long long out[NR];        // element offset of the row's output, -1: none
+  uint32_t mask[NR][8];
+};
+
+template <int NR>
+struct TreeShared {
+  uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2], q_empty[2];
+  uint64_t piece_full[TT_PIECES], piece_empty[TT_PIECES], row_full[TT_PIECES], drain;
+  TreePiece piece[TT_PIECES];
+  TreeRows<NR> rows[TT_PIECES];
+  uint32_t tmem, abort, last;
+  uint32_t odd[8];              // drafted positions whose V holds an infinity or NaN
+  long long scan[12], begin, end;
+  int begin_s, begin_n;         // the run's first request and the tiles of it that lie before
+  alignas(16) float lim[NR];    // a score above it raises its row's reference
+  alignas(16) float base[NR];   // the reference (0 where a row has seen nothing)
+  alignas(16) float fac[NR];    // what a rise takes off; at the end 1 / the sum
+  float ref[NR];                // the reference, -inf where a row has seen nothing
+  float red[4][NR];
+};
+
+// What an item's size follows from. A request without positions has one (empty) tile an item, which
+// gives its rows their zeros.
+struct TreeRequest {
+  int lo, rows, len, keys;
+  int row_tiles, tiles;  // items a K and V head; tiles an item
+};
+
+template <int NR>
+__device__ __forceinline__ TreeRequest tree_request(const AttendTreeArgs &a, int s) {
+  TreeRequest r;
+  r.lo = a.row_start ? a.row_start[s] : s;
+  r.rows = min(a.row_start ? a.row_start[s + 1] - r.lo : 1, a.max_rows);
+  if (r.lo < 0 || r.rows < 0) r.rows = 0;
+  r.len = max(a.lens[s], 0);
+  r.keys = int(min((long long)r.len + (a.mask ? r.rows : 0), (long long)a.width * a.bs));
+  r.row_tiles = (r.rows * (a.heads / a.kv_heads) + NR - 1) / NR;
+  r.tiles = max((r.keys + TT_KEYS - 1) / TT_KEYS, 1);
+  return r;
+}
+
+template <int HDP, int NR, bool WIDE>
+__global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HDP, NR, WIDE>::kCtas)
     attend_tree_kernel(const __grid_constant__ CUtensorMap map, const AttendTreeArgs a) {
-  using T = TreeTile<HDP, MT, WIDE>;
+  using T = TreeTile<HDP, NR, WIDE>;
   using E = typename std::conditional<WIDE, float, __half>::type;
-  constexpr int KS = HDP / 16, NT = T::kKeys / 8, ST = T::kStages;
+  constexpr int D = T::kRing, SOFT = T::kSoft, R = T::kRows;
+  constexpr int W_LOAD = SOFT / 32, W_MMA = W_LOAD + 1, W_ROWS = W_LOAD + 2, WARPS = W_LOAD + 3;
   extern __shared__ uint8_t raw[];
-  uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[ST], empty[ST];
-  __shared__ uint32_t info[ST];  // bit b: box b is in the pool; bit 31: every row sees all of it
-  __shared__ uint32_t abort_flag;
-  __shared__ float sh_m[T::kWK][MT], sh_l[T::kWK][MT];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  TreeShared<NR> &sh = *reinterpret_cast<TreeShared<NR> *>(smem + T::kOffBar);
   const int tid = int(threadIdx.x), lane = tid & 31, w = int(warp_id());
-  const int split = int(blockIdx.x) % a.splits, r0 = int(blockIdx.x) / a.splits * MT;
-  const int kvh = int(blockIdx.y), s = int(blockIdx.z), group = a.heads / a.kv_heads;
-  const Abort ab{&abort_flag, a.err};
+  const int group = a.heads / a.kv_heads;
+  const Abort ab{&sh.abort, a.err};
   if (tid == 0) {
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], TT_WARPS);
+    for (int i = 0; i < D; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
     }
-    abort_flag = 0u;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], W_LOAD);
+      mbar_init(&sh.pv_done[i], 1);
+      mbar_init(&sh.q_full[i], 1);
+      mbar_init(&sh.q_empty[i], 1);
+    }
+    for (int i = 0; i < TT_PIECES; ++i) {
+      mbar_init(&sh.piece_full[i], 1);
+      mbar_init(&sh.piece_empty[i], 1);
+      mbar_init(&sh.row_full[i], 1);
+    }
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0u;
+    sh.begin = sh.end = 0;
     fence_mbar_init();
     prefetch_tmap(&map);
   }
+  if (tid < 8) sh.odd[tid] = 0u;
+  if (w == W_MMA) {
+    tmem_alloc(&sh.tmem, T::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   griddep_launch_dependents();
   griddep_wait();  // the previous kernel of the stream has completed (programmatic launch)
+  const uint32_t tmem = sh.tmem;
+
+  // ---- this CTA's run: tiles begin .. end of all ---------------------------------------------------
+  const int per = (a.n + T::kThreads - 1) / T::kThreads;
+  const int s_lo = min(tid * per, a.n), s_hi = min(s_lo + per, a.n);
+  long long mine = 0;
+  for (int s = s_lo; s < s_hi; ++s) {
+    const TreeRequest r = tree_request<NR>(a, s);
+    mine += (long long)r.row_tiles * a.kv_heads * r.tiles;
+  }
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  if (lane == 31) sh.scan[w] = upto;
   __syncthreads();
-
-  const int lo = a.row_start ? a.row_start[s] : s;
-  const int t = min(a.row_start ? a.row_start[s + 1] - lo : 1, a.max_rows);
-  const int rows = t * group;  // of this K and V head: token by token, the heads of each together
-  if (r0 >= rows || lo < 0) return;
-  const int len = max(a.lens[s], 0);
-  const int keys = int(min((long long)len + (a.mask ? t : 0), (long long)a.width * a.bs));
-  const int k0 = split * a.chunk, k1 = min(keys, k0 + a.chunk);
-  const int n_tiles = k1 > k0 ? (k1 - k0 + TT_KEYS - 1) / TT_KEYS : 0;
-
-  if (w == TT_WARPS) {  // the producer
-    const int box = min(a.bs, TT_KEYS), boxes = TT_KEYS / box;
-    const int *table = a.table + (long long)s * a.width;
-    int i = 0;
-    for (; i < n_tiles; ++i) {
-      const int st = i % ST, pos = k0 + i * TT_KEYS + lane * box;
-      int b = -1;
-      if (lane < boxes && pos < keys) b = table[pos / a.bs];
-      const bool in = b >= 0 && b < a.blocks;
-      const uint32_t bits = __ballot_sync(0xffffffffu, in);
-      if (i >= ST && !mbar_wait_warp(&empty[st], ((i / ST) - 1) & 1, ab, kErrTimeoutProducer)) break;
-      if (lane == 0) {
-        const bool all = bits == (boxes == 32 ? ~0u : (1u << boxes) - 1u) &&
-                         k0 + (i + 1) * TT_KEYS <= min(len, keys);
-        info[st] = bits | (all ? 1u << 31 : 0u);
-        mbar_arrive_expect_tx(&full[st], T::kStage);
+  long long total = 0;
+  for (int k = 0; k < WARPS; ++k) {
+    if (k < w) upto += sh.scan[k];
+    total += sh.scan[k];
+  }
+  const int runs = int(min((long long)gridDim.x, total));
+  if (int(blockIdx.x) < runs) {
+    // A boundary inside a short item moves to the item's end.
+    for (int side = 0; side < 2; ++side) {
+      const long long at = total * (blockIdx.x + side) / runs;
+      if (side == 1 && at == total) {
+        if (tid == 0) sh.end = total;
+      } else if (at >= upto - mine && at < upto) {
+        long long left = at - (upto - mine);
+        int s = s_lo;
+        TreeRequest r = tree_request<NR>(a, s);
+        long long all = (long long)r.row_tiles * a.kv_heads * r.tiles;
+        while (left >= all) {
+          left -= all;
+          r = tree_request<NR>(a, ++s);
+          all = (long long)r.row_tiles * a.kv_heads * r.tiles;
+        }
+        const int into = int(left % r.tiles);
+        const int move = into && r.tiles <= TT_WHOLE ? r.tiles - into : 0;
+        if (side == 0) {
+          sh.begin = at + move;
+          sh.begin_s = s;
+          sh.begin_n = int(left + move);
+        } else {
+          sh.end = at + move;
+        }
       }
+    }
+  }
+  __syncthreads();
+  const int n = int(sh.end - sh.begin);  // tiles of this run
+
+  if (w == W_LOAD) {
+    // ---- loads: a lane a page of the tile. The ring takes them in the order in which the UMMAs do:
+    // K0, K1, V0, K2, V1, ..., V(n-1). This warp also cuts the run into items for the others.
+    const int box = min(a.bs, TT_KEYS), boxes = TT_KEYS / box;
+    int s = sh.begin_s;
+    TreeRequest r = {};
+    const int *table = nullptr;
+    int item = 0, tile = 0, items = 0;  // item of the request, tile of the item
+    const auto enter = [&](int at) {
+      s = at;
+      r = tree_request<NR>(a, s);
+      items = r.row_tiles * a.kv_heads;
+      table = a.table + (long long)s * a.width;
+    };
+    const auto block_of = [&](int t) {
+      const int p = t * TT_KEYS + lane * box;
+      const int b = lane < boxes && p < r.keys ? table[p / a.bs] : -1;
+      return b < 0 || b >= a.blocks ? a.blocks : b;  // past the tensor's end: zeros
+    };
+    if (n > 0) {
+      enter(s);
+      item = sh.begin_n / r.tiles;
+      tile = sh.begin_n % r.tiles;
+    }
+    int p = 0, k = 0, z = 0, z_next = 0, zv = 0, yv = 0, hv = 0;
+    bool ok = true, fresh = true, ahead = false;
+    const auto load = [&](int y, int head, int block) {
+      const int slot = p % D;
+      ok = p < D || mbar_wait_warp(&sh.empty[slot], (p / D - 1) & 1, ab, kErrTimeoutProducer);
+      if (!ok) return;
+      if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], T::kSlot);
       __syncwarp();
       if (lane < boxes) {
-        // A position outside the pool reads as zeros: block `blocks` is past the tensor's end.
-        uint8_t *to = tiles + st * T::kStage + lane * box * 128;
-        const int z = in ? b : a.blocks;
+        uint8_t *to = smem + slot * T::kSlot + lane * box * 128;
 #pragma unroll
-        for (int h = 0; h < HDP / 64; ++h) {
-          tma_load_4d(to + h * TT_HALF, &map, &full[st], 64 * h, pos % a.bs, kvh, z);
-          tma_load_4d(to + (HDP / 64 + h) * TT_HALF, &map, &full[st], 64 * h, pos % a.bs,
-                      a.kv_heads + kvh, z);
+        for (int h = 0; h < HDP / 64; ++h)
+          tma_load_4d(to + h * TT_HALF, &map, &sh.full[slot], 64 * h, y, head, block);
+      }
+      ++p;
+    };
+    for (int g = 0; g <= n && n > 0; ++g) {
+      const int z_v = z, y_v = yv, h_v = hv;
+      if (g < n) {
+        while (tile == r.tiles || item >= items) {  // on to the next item, past requests without rows
+          if (tile == r.tiles) tile = 0, ++item;
+          if (item >= items) {
+            enter(s + 1);
+            item = 0;
+          }
+          fresh = true;
         }
+        const int kvh = item / r.row_tiles;
+        if (fresh) {
+          if (k >= TT_PIECES &&
+              !mbar_wait_warp(&sh.piece_empty[k % TT_PIECES], (k / TT_PIECES - 1) & 1, ab,
+                              kErrTimeoutProducer))
+            break;
+          if (lane == 0) {
+            TreePiece q;
+            q.s = s;
+            q.kvh = kvh;
+            q.r0 = (item - kvh * r.row_tiles) * NR;
+            q.here = min(r.rows * group - q.r0, NR);
+            q.lo = r.lo;
+            q.rows = r.rows;
+            q.len = r.len;
+            q.keys = r.keys;
+            q.tile0 = tile;
+            q.tiles = min(r.tiles - tile, n - g);
+            q.slot = -1;
+            q.first = q.parts = 0;
+            if (q.tiles < r.tiles) {
+              // Run c holds tile x where c = ((x + 1) runs - 1) / total, rounded down.
+              const long long x0 = sh.begin + g - tile, x1 = x0 + r.tiles - 1;
+              q.first = int(((x0 + 1) * runs - 1) / total);
+              q.parts = int(((x1 + 1) * runs - 1) / total) - q.first + 1;
+              q.slot = 2 * int(blockIdx.x) + (tile == 0 ? 1 : 0);
+            }
+            sh.piece[k % TT_PIECES] = q;
+            mbar_arrive(&sh.piece_full[k % TT_PIECES]);
+          }
+          ++k;
+          fresh = false;
+          ahead = false;
+        }
+        z = ahead ? z_next : block_of(tile);
+        ahead = tile + 1 < r.tiles;
+        if (ahead) z_next = block_of(tile + 1);
+        yv = (tile * TT_KEYS + lane * box) % a.bs;
+        hv = kvh;
+        zv = z;
+        load(yv, hv, zv);
+        if (!ok) break;
+        ++tile;
+      }
+      if (g > 0) {
+        load(y_v, a.kv_heads + h_v, z_v);
+        if (!ok) break;
       }
     }
     // The shared memory stays until the last loads have landed, also where a wait gave up.
-    for (int j = max(i - ST, 0); j < i; ++j)
-      for (int k = 0; k < 2000 && !mbar_try_wait_sleep(&full[j % ST], (j / ST) & 1, 100000u); ++k) {}
-    return;
-  }
-
-  const int wr = w % T::kWR, wk = w / T::kWR;
-  const int g = lane >> 2, c2 = (lane & 3) * 2;
-  // This thread's rows r and r + 8 of the CTA's.
-  int row[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int r = r0 + wr * 16 + g + 8 * u, i = r / group;
-    row[u] = r < rows && lo + i < a.rows ? lo + i : -1;
-  }
-  uint32_t qh[KS][4], ql[WIDE ? KS : 1][4];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int u = x & 1, c = 16 * ks + c2 + 8 * (x >> 1);
-      const int head = kvh * group + (r0 + wr * 16 + g + 8 * u) % group;
-      E v[2] = {E(0.0f), E(0.0f)};
-      if (row[u] >= 0 && c < a.hd) {
-        const E *p = static_cast<const E *>(a.q) + row[u] * a.q_stride + head * a.hd + c;
-        v[0] = p[0];
-        v[1] = p[1];
-      }
-      if constexpr (WIDE) split2(v[0], v[1], qh[ks][x], ql[ks][x]);
-      else qh[ks][x] = uint32_t(__half_as_ushort(v[0])) | uint32_t(__half_as_ushort(v[1])) << 16;
-    }
-  float acc[2 * KS][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  const float scale = a.scale * 1.4426950408889634f;  // exponentials of base 2
-  bool ok = true;
-  for (int i = 0; i < n_tiles; ++i) {
-    const int st = i % ST;
-    ok = mbar_wait_warp(&full[st], (i / ST) & 1, ab, kErrTimeoutConsumer);
-    if (!ok) break;
-    const uint32_t kb = smem_u32(tiles + st * T::kStage), vb = kb + (HDP / 64) * TT_HALF;
-    const uint32_t bits = info[st];
-    const int first = wk * T::kKeys;  // the warp's first position in the tile
-    const int p0 = k0 + i * TT_KEYS + first;
-    float sc[NT][4] = {};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int n = 0; n < NT / 2; ++n) {
-        uint32_t b[4];
-        ldsm4(b, kb + tile_at(first + n * 16 + (lane >> 4) * 8 + (lane & 7),
-                              2 * ks + ((lane >> 3) & 1)));
-        mma16(sc[2 * n], qh[ks], b[0], b[1]);
-        mma16(sc[2 * n + 1], qh[ks], b[2], b[3]);
-        if constexpr (WIDE) {
-          mma16(sc[2 * n], ql[ks], b[0], b[1]);
-          mma16(sc[2 * n + 1], ql[ks], b[2], b[3]);
-        }
-      }
-    bool odd = false;  // a V row that some rows do not see holds an infinity or NaN
-    if (!(bits >> 31)) {
-      // Positions past the end, outside the pool, or drafted off a row's path.
-      const int box = min(a.bs, TT_KEYS);
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int j = first + 8 * n + c2 + (x & 1), p = k0 + i * TT_KEYS + j, d = p - len;
-          bool see = p < k1 && ((bits >> (j / box)) & 1u);
-          if (see && d >= 0)
-            see = row[x >> 1] >= 0 && d < 32 * a.words &&
-                  ((a.mask[(long long)row[x >> 1] * a.words + (d >> 5)] >> (d & 31)) & 1u);
-          if (!see) sc[n][x] = -INFINITY;
-        }
-      // What lies in a page past the end is nobody's: zeros in V (0 times NaN is not 0).
-      if (p0 + T::kKeys > k1) {
-        const int from = max(k1 - p0, 0);
-        for (int e = lane; e < (T::kKeys - from) * (HDP / 8); e += 32) {
-          const uint32_t at = vb + tile_at(first + from + e / (HDP / 8), e % (HDP / 8));
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
-        }
-        __syncwarp();
-      }
-      if (p0 + T::kKeys > len) {
-        bool bad = false;
-        for (int e = lane; e < T::kKeys * (HDP / 8); e += 32) {
-          uint32_t v[4];
-          const uint32_t at = vb + tile_at(first + e / (HDP / 8), e % (HDP / 8));
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                       : "r"(at)
-                       : "memory");
-#pragma unroll
-          for (int k = 0; k < 4; ++k) bad = bad || finite2(v[k]) != v[k];
-        }
-        odd = __any_sync(0xffffffffu, bad);
-      }
-    }
-    // The running maximum and sum, two rows a thread (four threads a row).
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float mx = m[u];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * u], sc[n][2 * u + 1]) * scale);
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float base = mx == -INFINITY ? 0.0f : mx;
-      const float carry = ex2(m[u] - base);
-      m[u] = mx;
-      float sum = 0.0f;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 2 * u; x < 2 * u + 2; ++x) {
-          sc[n][x] = ex2(fmaf(sc[n][x], scale, -base));
-          sum += sc[n][x];
-        }
-      l[u] = fmaf(l[u], carry, sum);
-      if (__any_sync(0xffffffffu, carry != 1.0f))
-#pragma unroll
-        for (int n = 0; n < 2 * KS; ++n) {
-          acc[n][2 * u] *= carry;
-          acc[n][2 * u + 1] *= carry;
-        }
-    }
-    const auto values = [&](auto clean) {
-#pragma unroll
-      for (int kk = 0; kk < NT / 2; ++kk) {
-        uint32_t ph[4], pl[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float p = sc[2 * kk + (x >> 1)][2 * (x & 1)], q = sc[2 * kk + (x >> 1)][2 * (x & 1) + 1];
-          if constexpr (WIDE) split2(p, q, ph[x], pl[x]);
-          else ph[x] = pack_half2(p, q);
-        }
-#pragma unroll
-        for (int n = 0; n < KS; ++n) {
-          uint32_t b[4];
-          ldsm4_t(b, vb + tile_at(first + kk * 16 + (lane & 15), 2 * n + (lane >> 4)));
-          if constexpr (decltype(clean)::value)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) b[x] = finite2(b[x]);
-          mma16(acc[2 * n], ph, b[0], b[1]);
-          mma16(acc[2 * n + 1], ph, b[2], b[3]);
-          if constexpr (WIDE) {
-            mma16(acc[2 * n], pl, b[0], b[1]);
-            mma16(acc[2 * n + 1], pl, b[2], b[3]);
+    for (int q = max(p - D, 0); q < p; ++q)
+      for (int i = 0; i < 2000 && !mbar_try_wait_sleep(&sh.full[q % D], (q / D) & 1, 100000u); ++i) {}
+  } else if (w == W_MMA) {
+    // ---- UMMAs: S of a tile, then P.V of the one before it ---------------------------------------
+    if (lane == 0 && n > 0) {
+      const uint64_t dq = sdesc_sw128(smem_u32(smem + T::kOffQ), 16, 1024);
+      const uint64_t dk = sdesc_sw128(smem_u32(smem), 16, 1024);
+      // With heads of 64 lanes 64.. multiply what lies behind V in shared memory; nobody reads them.
+      const uint64_t dv = sdesc_sw128(smem_u32(smem), TT_HALF, 1024);
+      const uint64_t dp = sdesc_sw128(smem_u32(smem + T::kOffP), TT_HALF, 1024);
+      int p = 0, k = -1, left = 0;
+      uint32_t cols = 0, cols_v = 0;
+      bool first = false, first_v = false, ok = true;
+      for (int g = 0; g <= n; ++g) {
+        cols_v = cols;
+        first_v = first;
+        if (g < n) {
+          first = left == 0;
+          if (first) {
+            ++k;
+            if (!mbar_wait(&sh.piece_full[k % TT_PIECES], (k / TT_PIECES) & 1, ab, kErrTimeoutMma))
+              break;
+            cols = uint32_t(sh.piece[k % TT_PIECES].here + 15) / 16 * 16;
+            left = sh.piece[k % TT_PIECES].tiles;
+            if (!mbar_wait(&sh.q_full[k % T::kQBufs], (k / T::kQBufs) & 1, ab, kErrTimeoutMma)) break;
           }
+          const int slot = p % D;
+          if (!mbar_wait(&sh.full[slot], (p / D) & 1, ab, kErrTimeoutMma)) break;
+          ++p;
+          tc_fence_after();
+          const uint32_t id = idesc_f16(TT_KEYS, cols, 0);
+          const uint64_t kd = dk + uint64_t(slot * T::kSlot >> 4);
+          const uint64_t qd = dq + uint64_t((k % T::kQBufs) * T::kParts * T::kQ >> 4);
+#pragma unroll
+          for (int part = 0; part < T::kParts; ++part)
+#pragma unroll
+            for (int kk = 0; kk < HDP / 16; ++kk)
+              umma_f16(tmem + (g & 1) * NR, kd + (((kk >> 2) * TT_HALF + (kk & 3) * 32) >> 4),
+                       qd + ((part * T::kQ + (kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), id,
+                       part + kk > 0 ? 1u : 0u);
+          umma_commit(&sh.s_full[g & 1]);
+          umma_commit(&sh.empty[slot]);
+          if (--left == 0) umma_commit(&sh.q_empty[k % T::kQBufs]);
+        }
+        if (g > 0) {
+          const int j = g - 1, slot = p % D;
+          if (!(ok = mbar_wait(&sh.full[slot], (p / D) & 1, ab, kErrTimeoutMma) &&
+                     mbar_wait(&sh.p_full[j & 1], (j >> 1) & 1, ab, kErrTimeoutMma)))
+            break;
+          ++p;
+          tc_fence_after();
+          const uint32_t id = idesc_f16(TT_KEYS, cols_v, 1) | (1u << 15);  // V^T: A is MN-major
+          const uint64_t vd = dv + uint64_t(slot * T::kSlot >> 4);
+          const uint64_t pd = dp + uint64_t((j % T::kPBufs) * T::kParts * T::kP >> 4);
+#pragma unroll
+          for (int part = 0; part < T::kParts; ++part)
+#pragma unroll
+            for (int kk = 0; kk < TT_KEYS / 16; ++kk)
+              umma_f16(tmem + 2 * NR, vd + uint64_t(kk * 16 * 128 >> 4),
+                       pd + uint64_t((part * T::kP + kk * 16 * 128) >> 4), id,
+                       !first_v || part + kk > 0 ? 1u : 0u);
+          umma_commit(&sh.pv_done[j & 1]);
+          umma_commit(&sh.empty[slot]);
         }
       }
-    };
-    if (!odd) {
-      values(std::false_type());
-    } else {
-      // Infinities and NaN in V go one by one to the rows that see them, and the products get
-      // zeros in their place (0 times infinity is not 0).
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-          const int from = (lane & ~3) | (j >> 1);
-          float p[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float e = __shfl_sync(0xffffffffu, sc[n][2 * u], from);
-            const float f = __shfl_sync(0xffffffffu, sc[n][2 * u + 1], from);
-            p[u] = (j & 1) ? f : e;
-          }
-#pragma unroll
-          for (int c = 0; c < 2 * KS; ++c) {
-            uint32_t v;
-            asm volatile("ld.shared.b32 %0, [%1];"
-                         : "=r"(v)
-                         : "r"(vb + tile_at(first + 8 * n + j, c) + 2 * c2)
-                         : "memory");
-            const uint32_t rest = v ^ finite2(v);
-            if (rest == 0u) continue;
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&rest));
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              if (p[u] != 0.0f) {
-                acc[c][2 * u] = fmaf(p[u], f.x, acc[c][2 * u]);
-                acc[c][2 * u + 1] = fmaf(p[u], f.y, acc[c][2 * u + 1]);
-              }
-          }
-        }
-      values(std::true_type());
+      // TMEM and shared memory stay until the last UMMA is done, also where a wait gave up.
+      umma_commit(&sh.drain);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(&sh.drain, 0) && clock64() - t0 < kWaitCycles) {
+      }
     }
-    if (!(bits >> 31)) fence_proxy_async_smem();  // the zeros, before a later load
     __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[st]);
-  }
+  } else if (w == W_ROWS) {
+    // ---- an item's rows: where they go, what they see, and Q into shared memory ------------------
+    const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (a.q_stride * sizeof(E))) & 15u) == 0;
+    for (int k = 0, done = 0; done < n; ++k) {
+      const int pc = k % TT_PIECES, qb = k % T::kQBufs;
+      if (!mbar_wait_warp(&sh.piece_full[pc], (k / TT_PIECES) & 1, ab, kErrTimeoutConsumer)) break;
+      const TreePiece &q = sh.piece[pc];
+      TreeRows<NR> &to = sh.rows[pc];
+      done += q.tiles;
+      for (int r = lane; r < NR; r += 32) {
+        const int i = (q.r0 + r) / group, head = q.kvh * group + (q.r0 + r) - i * group;
+        const bool live = r < q.here && q.lo + i < a.rows;
+        const long long row = q.lo + i;
+        to.out[r] = !live ? -1
+                    : q.slot < 0 ? row * a.o_stride + (long long)head * a.hd
+                                 : ((long long)q.slot * NR + r) * (a.hd + 4);
+        for (int x = 0; x < a.words; ++x)
+          to.mask[r][x] = live ? a.mask[row * a.words + x] : 0u;
+      }
+      if (k >= T::kQBufs &&
+          !mbar_wait_warp(&sh.q_empty[qb], (k / T::kQBufs - 1) & 1, ab, kErrTimeoutConsumer))
+        break;
+      uint8_t *base = smem + T::kOffQ + qb * T::kParts * T::kQ;
+      // Eight elements a lane and step, four steps in flight; rows to the next 16 are zeros.
+      const int chunks = (q.here + 15) / 16 * 16 * (HDP / 8);
+      for (int e0 = lane; e0 < chunks; e0 += 128) {
+        E v[4][8];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-  }
+        for (int u = 0; u < 4; ++u) {
+          const int e = e0 + 32 * u, r = e / (HDP / 8), c = e % (HDP / 8);
+          const int i = (q.r0 + r) / group, head = q.kvh * group + (q.r0 + r) - i * group;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[u][x] = E(0.0f);
+          if (e < chunks && r < q.here && q.lo + i < a.rows && c * 8 < a.hd) {
+            const E *from = static_cast<const E *>(a.q) + (long long)(q.lo + i) * a.q_stride +
+                            head * a.hd + c * 8;
+            if (vec) {
+#pragma unroll
+              for (int x = 0; x < int(sizeof(E)) / 2; ++x)
+                reinterpret_cast<uint4 *>(v[u])[x] = reinterpret_cast<const uint4 *>(from)[x];
+            } else {
+#pragma unroll
+              for (int x = 0; x < 8; ++x) v[u][x] = from[x];
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int e = e0 + 32 * u, r = e / (HDP / 8), c = e % (HDP / 8);
+          if (e >= chunks) break;
+          uint8_t *at = base + (c >> 3) * NR * 128 + sw128_offset(r, c & 7);
+          if constexpr (WIDE) {
+            uint32_t hi[4], low[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) split2(v[u][2 * x], v[u][2 * x + 1], hi[x], low[x]);
+            *reinterpret_cast<uint4 *>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4 *>(at + T::kQ) = make_uint4(low[0], low[1], low[2], low[3]);
+          } else {
+            *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(v[u]);
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh.row_full[pc]);
+        mbar_arrive(&sh.q_full[qb]);
+      }
+    }
+  } else {
+    // ---- softmax: a position a thread, the warps of a group the rows from col0 on ------------------
+    const auto sync = [] { asm volatile("barrier.cta.sync 1, %0;" ::"n"(SOFT) : "memory"); };
+    const auto any = [](bool x) {  // a barrier that says whether any thread holds x
+      uint32_t r;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.u32 p, %1, 0;\n\t"
+          "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t}\n"
+          : "=r"(r)
+          : "r"(uint32_t(x)), "n"(SOFT)
+          : "memory");
+      return r != 0;
+    };
+    const int key = tid & 127, quarter = w & 3, col0 = (w >> 2) * R;
+    const uint32_t lanes = tmem + (uint32_t(quarter) * 32u << 16) + col0;
+    const float scale = a.scale * 1.4426950408889634f;  // exponentials of base 2
+    int pv = 0;  // V's place in the ring
+    for (int k = 0, g = 0; g < n; ++k) {
+      const int pc = k % TT_PIECES;
+      // Where a wait gives up, all warps leave together; inside an item they run on (later waits give
+      // up soon): the barriers need them all.
+      bool ok = mbar_wait_warp(&sh.row_full[pc], (k / TT_PIECES) & 1, ab, kErrTimeoutConsumer);
+      if (any(!ok)) break;
+      const TreePiece &q = sh.piece[pc];
+      const TreeRows<NR> &rows = sh.rows[pc];
+      const int here = q.here, tiles = q.tiles;
+      const int *table = a.table + (long long)q.s * a.width;
+      for (int r = tid; r < NR; r += SOFT) {
+        sh.ref[r] = -INFINITY;
+        sh.base[r] = 0.0f;
+        sh.lim[r] = rows.out[r] >= 0 ? -INFINITY : INFINITY;
+      }
+      float l[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) l[r] = 0.0f;
+      const auto entry = [&](int pos) { return pos < q.keys ? table[pos / a.bs] : -1; };
+      int b = entry(q.tile0 * TT_KEYS + key);
+      sync();
+      for (int i = 0; i < tiles; ++i, ++g) {
+        const int pos = (q.tile0 + i) * TT_KEYS + key, d = pos - q.len;
+        const bool there = b >= 0 && b < a.blocks;  // below q.keys and in the pool
+        if (i + 1 < tiles) b = entry(pos + TT_KEYS);
+        const bool all = __all_sync(0xffffffffu, there && d < 0);  // every row sees the warp's
+        // What this position is seen by, a bit a row.
+        uint32_t vis[(R + 31) / 32];
+        if (!all) {
+#pragma unroll
+          for (int x = 0; x < (R + 31) / 32; ++x) {
+            vis[x] = there ? ~0u : 0u;
+            if (there && d >= 0) {
+              vis[x] = 0u;
+              if (d < 32 * a.words)
+#pragma unroll
+                for (int r = 0; r < (R < 32 ? R : 32); ++r)
+                  vis[x] |= ((rows.mask[col0 + 32 * x + r][d >> 5] >> (d & 31)) & 1u) << r;
+            }
+          }
+        }
+        mbar_wait_warp(&sh.s_full[g & 1], (g >> 1) & 1, ab, kErrTimeoutConsumer);
+        tc_fence_after();
+        uint32_t u[R / 16][16];
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < R / 16; ++c)
+          if (col0 + 16 * c < here) tmem_ld16(lanes + (g & 1) * NR + 16 * c, u[c]);
+        tmem_wait_ld();
+        const auto x_of = [&](int r) -> float {
+          return __uint_as_float(u[r / 16][r % 16]);
+        };
+        bool rise = false;
+#pragma unroll
+        for (int c = 0; c < R / 16; ++c)
+          if (col0 + 16 * c < here) {
+            if (!all) {
+#pragma unroll
+              for (int y = 0; y < 16; ++y)
+                if (!((vis[c / 2] >> (16 * (c & 1) + y)) & 1u)) u[c][y] = 0xff800000u;  // -inf
+            }
+#pragma unroll
+            for (int y = 0; y < 16; y += 4) {
+              const float4 lim = *reinterpret_cast<const float4 *>(&sh.lim[col0 + 16 * c + y]);
+              const int r = 16 * c + y;
+              rise |= (x_of(r) > lim.x) | (x_of(r + 1) > lim.y) | (x_of(r + 2) > lim.z) |
+                      (x_of(r + 3) > lim.w);
+            }
+          }
+        if (any(rise)) {
+          // The tile's maximum of every row, and what is summed so far brought down to it.
+#pragma unroll
+          for (int c = 0; c < (R + 31) / 32; ++c)
+            if (col0 + 32 * c < here) {
+              float x[32];
+#pragma unroll
+              for (int y = 0; y < 32; ++y) {
+                const int r = 32 * c + y;
+                x[y] = r < R && col0 + r / 16 * 16 < here ? x_of(r % R) : -INFINITY;
+              }
+              const float top = lanes_reduce<true>(x);
+              if (32 * c + lane < R) sh.red[quarter][col0 + 32 * c + lane] = top;
+            }
+          sync();
+          for (int r = tid; r < here; r += SOFT) {
+            const float old = sh.ref[r];
+            const float top =
+                fmaxf(fmaxf(sh.red[0][r], sh.red[1][r]), fmaxf(sh.red[2][r], sh.red[3][r]));
+            const float ref = fmaxf(old, top * scale);
+            sh.fac[r] = ref == -INFINITY ? 1.0f : ex2(old - ref);
+            sh.ref[r] = ref;
+            sh.base[r] = ref == -INFINITY ? 0.0f : ref;
+            if (rows.out[r] >= 0) sh.lim[r] = (ref + TT_RISE) / scale;
+          }
+          sync();
+          if (i > 0) {
+            const int j = g - 1;
+            mbar_wait_warp(&sh.pv_done[j & 1], (j >> 1) & 1, ab, kErrTimeoutConsumer);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < R / 16; ++c)
+              if (col0 + 16 * c < here) {
+                uint32_t o[16];
+                __syncwarp();
+                tmem_ld16(lanes + 2 * NR + 16 * c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int y = 0; y < 16; ++y) {
+                  const float f = sh.fac[col0 + 16 * c + y];
+                  o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                  l[16 * c + y] *= f;
+                }
+                tmem_st16(lanes + 2 * NR + 16 * c, o);
+              }
+            tmem_wait_st();
+          }
+        }
+        // P is free once the product that read it is done.
+        if (g >= T::kPBufs) {
+          const int j = g - T::kPBufs;
+          mbar_wait_warp(&sh.pv_done[j & 1], (j >> 1) & 1, ab, kErrTimeoutConsumer);
+        }
+        uint8_t *to = smem + T::kOffP + (g % T::kPBufs) * T::kParts * T::kP;
+#pragma unroll
+        for (int c = 0; c < R / 16; ++c)
+          if (col0 + 16 * c < here) {
+            uint32_t hi[8], low[8];
+#pragma unroll
+            for (int y = 0; y < 16; y += 4) {
+              const float4 base = *reinterpret_cast<const float4 *>(&sh.base[col0 + 16 * c + y]);
+              const int r = 16 * c + y;
+              const float x0 = ex2(fmaf(x_of(r), scale, -base.x));
+              const float x1 = ex2(fmaf(x_of(r + 1), scale, -base.y));
+              const float x2 = ex2(fmaf(x_of(r + 2), scale, -base.z));
+              const float x3 = ex2(fmaf(x_of(r + 3), scale, -base.w));
+              l[r] += x0;
+              l[r + 1] += x1;
+              l[r + 2] += x2;
+              l[r + 3] += x3;
+              if constexpr (WIDE) {
+                split2(x0, x1, hi[y / 2], low[y / 2]);
+                split2(x2, x3, hi[y / 2 + 1], low[y / 2 + 1]);
+              } else {
+                hi[y / 2] = pack_half2(x0, x1);
+                hi[y / 2 + 1] = pack_half2(x2, x3);
+              }
+            }
+            const int cc = col0 / 16 + c;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              uint8_t *at = to + (cc >> 2) * TT_HALF + sw128_offset(key, 2 * (cc & 3) + y);
+              *reinterpret_cast<uint4 *>(at) =
+                  make_uint4(hi[4 * y], hi[4 * y + 1], hi[4 * y + 2], hi[4 * y + 3]);
+              if constexpr (WIDE)
+                *reinterpret_cast<uint4 *>(at + T::kP) =
+                    make_uint4(low[4 * y], low[4 * y + 1], low[4 * y + 2], low[4 * y + 3]);
+            }
+          }
+        // What a row does not see must not reach it through 0 times infinity: V is zero past the
+        // end, and a drafted position's infinities and NaN are zeros here and added at the end to the
+        // rows that see them.
+        pv = g == n - 1 ? 2 * n - 1 : 2 * g + 2;
+        if (!all && col0 == 0) {
+          mbar_wait_warp(&sh.full[pv % D], (pv / D) & 1, ab, kErrTimeoutConsumer);
+          uint8_t *v = smem + (pv % D) * T::kSlot;
+          if (!there || d >= 0) {
+            bool odd = false;
+#pragma unroll 2
+            for (int c = 0; c < HDP / 8; ++c) {
+              uint4 *at = reinterpret_cast<uint4 *>(v + (c >> 3) * TT_HALF + sw128_offset(key, c & 7));
+              const uint4 x = *at;
+              uint4 y = make_uint4(0u, 0u, 0u, 0u);
+              if (there) y = make_uint4(finite2(x.x), finite2(x.y), finite2(x.z), finite2(x.w));
+              if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+                *at = y;
+                odd = true;
+              }
+            }
+            if (there && odd && d < 256) atomicOr(&sh.odd[d >> 5], 1u << (d & 31));
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[g & 1]);
+      }
 
-  // The warps' shares of the positions meet in shared memory, over the tiles.
-  float *sum = reinterpret_cast<float *>(tiles);  // [kWK][MT][HDP]
-  warps_sync();
+      // ---- the item's sums, and its rows out ---------------------------------------------------------
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int r = wr * 16 + g + 8 * u;
-    if ((lane & 3) == 0) {
-      sh_m[wk][r] = m[u];
-      sh_l[wk][r] = l[u];
+      for (int c = 0; c < (R + 31) / 32; ++c) {
+        float x[32];
+#pragma unroll
+        for (int y = 0; y < 32; ++y) x[y] = 32 * c + y < R ? l[(32 * c + y) % R] : 0.0f;
+        const float sum = lanes_reduce<false>(x);
+        if (32 * c + lane < R) sh.red[quarter][col0 + 32 * c + lane] = sum;
+      }
+      sync();
+      for (int r = tid; r < NR; r += SOFT) {
+        const float sum = sh.red[0][r] + sh.red[1][r] + sh.red[2][r] + sh.red[3][r];
+        sh.fac[r] = q.slot >= 0 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
+        if (q.slot >= 0 && rows.out[r] >= 0)
+          *reinterpret_cast<float2 *>(a.part + rows.out[r] + a.hd) = make_float2(sh.ref[r], sum);
+      }
+      ok = mbar_wait_warp(&sh.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, ab, kErrTimeoutConsumer);
+      const bool good = !any(!ok || ab.raised());
+      tc_fence_after();
+      uint32_t odd = 0u;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) odd |= sh.odd[x];
+      const int dim = quarter * 32 + lane;  // the TMEM lane is the element of the head
+      if (quarter * 32 < a.hd) {
+#pragma unroll 1
+        for (int c = 0; c < R / 16; ++c) {
+          if (col0 + 16 * c >= here) break;
+          uint32_t o[16];
+          __syncwarp();
+          tmem_ld16(lanes + 2 * NR + 16 * c, o);
+          tmem_wait_ld();
+          if (odd) {
+            for (int d = 0; d < min(q.rows, 256); ++d) {
+              if (!((sh.odd[d >> 5] >> (d & 31)) & 1u)) continue;
+              const int pos = q.len + d, blk = table[pos / a.bs];
+              const __half h = dim < a.hd ? a.pool[(((long long)blk * 2 + 1) * a.kv_heads + q.kvh) * a.bs * a.hd +
+                                                   (long long)(pos % a.bs) * a.hd + dim]
+                                          : __half(0.0f);
+              if ((__half_as_ushort(h) & 0x7c00u) != 0x7c00u) continue;
+#pragma unroll
+              for (int y = 0; y < 16; ++y)
+                if ((rows.mask[col0 + 16 * c + y][d >> 5] >> (d & 31)) & 1u)
+                  o[y] = __float_as_uint(__uint_as_float(o[y]) + __half2float(h));
+            }
+          }
+          long long at[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) at[y] = good && dim < a.hd ? rows.out[col0 + 16 * c + y] : -1;
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            const float v = __uint_as_float(o[y]) * sh.fac[col0 + 16 * c + y];
+            if (at[y] >= 0) {
+              if (q.slot < 0) static_cast<E *>(a.o)[at[y] + dim] = E(v);
+              else a.part[at[y] + dim] = v;
+            }
+          }
+        }
+      }
+      if (q.slot >= 0) {
+        // The run that brings the last part of an item joins them all.
+        __threadfence();
+        sync();
+        if (tid == 0) sh.last = atomicAdd(&a.count[q.first], 1) == q.parts - 1;
+        sync();
+        if (sh.last && good) {
+          __threadfence();
+          const auto part_of = [&](int x, int r) {
+            const long long slot = 2ll * (q.first + x) + (x == 0 ? 1 : 0);
+            return a.part + (slot * NR + r) * (a.hd + 4);
+          };
+          for (int r = tid; r < here; r += SOFT) {
+            float top = -INFINITY, sum = 0.0f;
+            for (int x = 0; x < q.parts; ++x) top = fmaxf(top, __ldcg(part_of(x, r) + a.hd));
+            const float base = top == -INFINITY ? 0.0f : top;
+            for (int x = 0; x < q.parts; ++x) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(x, r) + a.hd));
+              sum = fmaf(ex2(ml.x - base), ml.y, sum);
+            }
+            sh.base[r] = base;
+            sh.fac[r] = sum != 0.0f ? 1.0f / sum : 0.0f;
+          }
+          sync();
+          const int quads = a.hd / 4;
+          for (int e = tid; e < here * quads; e += SOFT) {
+            const int r = e / quads, c = (e - r * quads) * 4;
+            const int row = q.lo + (q.r0 + r) / group, head = q.kvh * group + (q.r0 + r) % group;
+            if (row >= a.rows) continue;
+            const float base = sh.base[r], inv = sh.fac[r];
+            float o[4] = {};
+#pragma unroll 4
+            for (int x = 0; x < q.parts; ++x) {
+              const float *from = part_of(x, r);
+              const float f = ex2(__ldcg(from + a.hd) - base);
+              const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + c));
+              o[0] = fmaf(f, v.x, o[0]);
+              o[1] = fmaf(f, v.y, o[1]);
+              o[2] = fmaf(f, v.z, o[2]);
+              o[3] = fmaf(f, v.w, o[3]);
+            }
+            E *to = static_cast<E *>(a.o) + row * a.o_stride + (long long)head * a.hd + c;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) to[x] = E(o[x] * inv);
+          }
+          if (tid == 0) a.count[q.first] = 0;  // for the next call
+        }
+      }
+      sync();  // the rows and references are read, the item's place is free
+      if (odd && tid < 8) sh.odd[tid] = 0u;
+      tc_fence_before();
+      if (tid == 0) mbar_arrive(&sh.piece_empty[pc]);
     }
-#pragma unroll
-    for (int n = 0; n < 2 * KS; ++n)
-      *reinterpret_cast<float2 *>(sum + (wk * MT + r) * HDP + 8 * n + c2) =
-          make_float2(acc[n][2 * u], acc[n][2 * u + 1]);
   }
-  warps_sync();
-  if (abort_flag) return;  // a wait gave up: the outputs are left as they are
-  const int quads = a.hd / 4;
-  for (int e = tid; e < MT * quads; e += TT_WARPS * 32) {
-    const int r = e / quads, c = (e - r * quads) * 4, rr = r0 + r;
-    if (rr >= rows) break;
-    const int q = lo + rr / group, head = kvh * group + rr % group;
-    if (q >= a.rows) break;
-    float top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < T::kWK; ++k) top = fmaxf(top, sh_m[k][r]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, o[4] = {};
-#pragma unroll
-    for (int k = 0; k < T::kWK; ++k) {
-      const float f = ex2(sh_m[k][r] - base);
-      const float4 v = *reinterpret_cast<const float4 *>(sum + (k * MT + r) * HDP + c);
-      total = fmaf(f, sh_l[k][r], total);
-      o[0] = fmaf(f, v.x, o[0]);
-      o[1] = fmaf(f, v.y, o[1]);
-      o[2] = fmaf(f, v.z, o[2]);
-      o[3] = fmaf(f, v.w, o[3]);
-    }
-    if (a.splits == 1) {
-      const float inv = total != 0.0f ? 1.0f / total : 0.0f;
-      E *to = static_cast<E *>(a.o) + q * a.o_stride + (long long)head * a.hd + c;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) to[x] = E(o[x] * inv);
-    } else {
-      float *to = a.part + (((long long)q * a.heads + head) * a.splits + split) * (a.hd + 4);
-      *reinterpret_cast<float4 *>(to + c) = make_float4(o[0], o[1], o[2], o[3]);
-      if (c == 0) *reinterpret_cast<float2 *>(to + a.hd) = make_float2(top, total);
-    }
-  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (w == W_MMA) tmem_dealloc(tmem, T::kCols);
 }
 
-// The ranges of a row joined: a CTA a (drafted row, request), four elements a thread.
-template <typename E>
-__global__ void __launch_bounds__(128) attend_tree_join_kernel(const AttendTreeArgs a) {
-  griddep_launch_dependents();
-  griddep_wait();  // the previous kernel of the stream has completed (programmatic launch)
-  const int i = int(blockIdx.x), s = int(blockIdx.z);
-  const int lo = a.row_start ? a.row_start[s] : s;
-  const int t = min(a.row_start ? a.row_start[s + 1] - lo : 1, a.max_rows), q = lo + i;
-  if (i >= t || lo < 0 || q >= a.rows) return;
-  const int quads = a.hd / 4;
-  for (int e = int(blockIdx.y * blockDim.x + threadIdx.x); e < a.heads * quads;
-       e += int(gridDim.y * blockDim.x)) {
-    const int head = e / quads, c = (e - head * quads) * 4;
-    const float *from = a.part + ((long long)q * a.heads + head) * a.splits * (a.hd + 4);
-    float top = -INFINITY;
-    for (int k = 0; k < a.splits; ++k) top = fmaxf(top, from[k * (a.hd + 4) + a.hd]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, o[4] = {};
-    for (int k = 0; k < a.splits; ++k) {
-      const float2 ml = *reinterpret_cast<const float2 *>(from + k * (a.hd + 4) + a.hd);
-      const float4 v = *reinterpret_cast<const float4 *>(from + k * (a.hd + 4) + c);
-      const float f = ex2(ml.x - base);
-      total = fmaf(f, ml.y, total);
-      o[0] = fmaf(f, v.x, o[0]);
-      o[1] = fmaf(f, v.y, o[1]);
-      o[2] = fmaf(f, v.z, o[2]);
-      o[3] = fmaf(f, v.w, o[3]);
-    }
-    const float inv = total != 0.0f ? 1.0f / total : 0.0f;
-    E *to = static_cast<E *>(a.o) + q * a.o_stride + (long long)head * a.hd + c;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) to[x] = E(o[x] * inv);
-  }
-}
-
-template <int HDP, int MT, bool WIDE>
-cudaError_t launch_tile(const CUtensorMap &map, const AttendTreeArgs &a, int row_tiles, int n,
-                        cudaStream_t s) {
-  auto *kernel = attend_tree_kernel<HDP, MT, WIDE>;
-  constexpr size_t smem = TreeTile<HDP, MT, WIDE>::kSmem;
+template <int HDP, int NR, bool WIDE>
+cudaError_t launch_tile(const CUtensorMap &map, const AttendTreeArgs &a, int sms, cudaStream_t s) {
+  auto *kernel = attend_tree_kernel<HDP, NR, WIDE>;
+  using T = TreeTile<HDP, NR, WIDE>;
+  constexpr size_t smem = T::kOffBar + sizeof(TreeShared<NR>) + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory");
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -452,48 +832,46 @@ cudaError_t launch_tile(const CUtensorMap &map, const AttendTreeArgs &a, int row
     if (e != cudaSuccess) return e;
     if (dev < 64) configured[dev] = true;
   }
-  return launch_pdl(kernel, dim3(a.splits * row_tiles, a.kv_heads, n), dim3(TT_THREADS), smem, s,
-                    map, a);
+  // No more runs than there can be tiles.
+  const long long items =
+      ((long long)a.max_rows * (a.heads / a.kv_heads) + NR - 1) / NR * a.kv_heads * a.n;
+  const long long tiles = items * std::max((a.max_len + TT_KEYS - 1) / TT_KEYS, 1);
+  const int grid = int(std::min<long long>((long long)sms * T::kCtas, tiles));
+  return launch_pdl(kernel, dim3(grid), dim3(T::kThreads), smem, s, map, a);
 }
 
-template <int HDP, bool WIDE>
-cudaError_t launch_rows(const CUtensorMap &map, const AttendTreeArgs &a, const AttendTreePlan &p,
-                        int n, cudaStream_t s) {
-  return p.row_tile == 16   ? launch_tile<HDP, 16, WIDE>(map, a, p.row_tiles, n, s)
-         : p.row_tile == 32 ? launch_tile<HDP, 32, WIDE>(map, a, p.row_tiles, n, s)
-                            : launch_tile<HDP, 64, WIDE>(map, a, p.row_tiles, n, s);
+template <int HDP>
+cudaError_t launch_rows(const CUtensorMap &map, const AttendTreeArgs &a, int f16, int sms,
+                        cudaStream_t s) {
+  switch (attend_tree_rows(a.max_rows, a.heads, a.kv_heads, f16)) {
+    case 16:
+      return f16 ? launch_tile<HDP, 16, false>(map, a, sms, s) : launch_tile<HDP, 16, true>(map, a, sms, s);
+    case 32:
+      return f16 ? launch_tile<HDP, 32, false>(map, a, sms, s) : launch_tile<HDP, 32, true>(map, a, sms, s);
+    case 64:
+      return f16 ? launch_tile<HDP, 64, false>(map, a, sms, s) : launch_tile<HDP, 64, true>(map, a, sms, s);
+    default:
+      return launch_tile<HDP, 128, false>(map, a, sms, s);
+  }
 }
 
 }  // namespace
 
-AttendTreePlan attend_tree_plan(int n, int max_rows, int max_len, int heads, int kv_heads, int sms) {
-  AttendTreePlan p;
+int attend_tree_rows(int max_rows, int heads, int kv_heads, int f16) {
   const long long rows = (long long)max_rows * (heads / kv_heads);
-  p.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  p.row_tiles = int((rows + p.row_tile - 1) / p.row_tile);
-  const long long ctas = (long long)n * kv_heads * p.row_tiles;
-  // Ranges of 256 positions at least, as many as fill the SMs four times.
-  const long long want = (4ll * sms + ctas - 1) / ctas;
-  const long long most = std::max<long long>(1, (max_len + 255) / 256);
-  p.splits = int(std::min<long long>(std::min(want, most), 128));
-  p.chunk = int(((long long)max_len + p.splits - 1) / p.splits);
-  p.chunk = std::max((p.chunk + TT_KEYS - 1) / TT_KEYS, 1) * TT_KEYS;
-  p.splits = std::max((max_len + p.chunk - 1) / p.chunk, 1);
-  return p;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || !f16 ? 64 : 128;
 }
 
-cudaError_t launch_attend_tree(const CUtensorMap &map, const AttendTreeArgs &a,
-                               const AttendTreePlan &p, int f16, int n, cudaStream_t s) {
-  if (n <= 0 || a.max_rows <= 0) return cudaSuccess;
-  cudaError_t e;
-  if (a.hd <= 64)
-    e = f16 ? launch_rows<64, false>(map, a, p, n, s) : launch_rows<64, true>(map, a, p, n, s);
-  else
-    e = f16 ? launch_rows<128, false>(map, a, p, n, s) : launch_rows<128, true>(map, a, p, n, s);
-  if (e != cudaSuccess || a.splits == 1) return e;
-  const dim3 grid(a.max_rows, std::min(8, (a.heads * a.hd / 4 + 127) / 128), n);
-  return f16 ? launch_pdl(attend_tree_join_kernel<__half>, grid, dim3(128), 0, s, a)
-             : launch_pdl(attend_tree_join_kernel<float>, grid, dim3(128), 0, s, a);
+size_t attend_tree_part_bytes(int max_rows, int heads, int kv_heads, int hd, int f16, int sms) {
+  // Two parts a run: of the item that it begins in, and of the one that it ends in.
+  return size_t(2) * kTreeRunsPerSm * sms * attend_tree_rows(max_rows, heads, kv_heads, f16) *
+         (hd + 4) * sizeof(float);
+}
+
+cudaError_t launch_attend_tree(const CUtensorMap &map, const AttendTreeArgs &a, int f16, int sms,
+                               cudaStream_t s) {
+  if (a.n <= 0 || a.max_rows <= 0) return cudaSuccess;
+  return a.hd <= 64 ? launch_rows<64>(map, a, f16, sms, s) : launch_rows<128>(map, a, f16, sms, s);
 }
 
 }  // namespace wv

@@ -27,7 +27,7 @@ struct wavo_ctx {
   int sms = 0;
   cudaStream_t own = nullptr;
   cudaStream_t stream = nullptr;
-  int *dev_err = nullptr;    // the kernels' error word
+  int *dev_err = nullptr;    // the kernels' error word, then attend_tree's counts (kTreeCounts on)
   void *ws = nullptr;        // scratch for casts and repacks
   size_t ws_bytes = 0;
   bool capturing = false;
@@ -279,6 +279,12 @@ wavo_status workspace(wavo_ctx *ctx, size_t bytes, void **out) {
   return WAVO_OK;
 }
 
+// The error word has a cache line of its own; the counts follow.
+constexpr int kTreeCounts = 32;
+size_t dev_words_bytes(const wavo_ctx *ctx) {
+  return (kTreeCounts + size_t(wv::kTreeRunsPerSm) * ctx->sms) * sizeof(int);
+}
+
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // IEEE binary16 from f32, round to nearest even (the reference GPU GEMM's rounding of W).
@@ -333,8 +339,8 @@ wavo_status wavo_create(int device, wavo_ctx **out) {
   ctx->sms = prop.multiProcessorCount;
   if ((e = cudaSetDevice(device)) != cudaSuccess ||
       (e = cudaStreamCreateWithFlags(&ctx->own, cudaStreamNonBlocking)) != cudaSuccess ||
-      (e = cudaMalloc(&ctx->dev_err, sizeof(int))) != cudaSuccess ||
-      (e = cudaMemset(ctx->dev_err, 0, sizeof(int))) != cudaSuccess) {
+      (e = cudaMalloc(&ctx->dev_err, dev_words_bytes(ctx))) != cudaSuccess ||
+      (e = cudaMemset(ctx->dev_err, 0, dev_words_bytes(ctx))) != cudaSuccess) {
     fail(nullptr, WAVO_ECUDA, "context setup: %s", cudaGetErrorString(e));
     if (ctx->own) cudaStreamDestroy(ctx->own);
     if (ctx->dev_err) cudaFree(ctx->dev_err);
@@ -443,7 +449,7 @@ wavo_status wavo_sync(wavo_ctx *ctx, uint32_t timeout_ms) {
   int code = 0;
   CK(cudaMemcpy(&code, ctx->dev_err, sizeof code, cudaMemcpyDeviceToHost), "error word");
   if (code) {
-    CK(cudaMemset(ctx->dev_err, 0, sizeof(int)), "error word reset");
+    CK(cudaMemset(ctx->dev_err, 0, dev_words_bytes(ctx)), "error word reset");
     static const char *what[] = {"", "TMA producer", "MMA issuer", "softmax/epilogue", "drain"};
     return fail(ctx, WAVO_EDEVICE, "a kernel's bounded wait gave up (%s, code %d)",
                 code > 0 && code < 5 ? what[code] : "?", code);
@@ -1537,7 +1543,7 @@ wavo_status wavo_attend(wavo_ctx *ctx, const float *q, const void *kv, float *pa
 
 namespace {
 
-// A paged cache as {hd, bs, 2 kv_heads, blocks} of f16, boxes of 64 elements x min(bs, 64) positions
+// A paged cache as {hd, bs, 2 kv_heads, blocks} of f16, boxes of 64 elements x min(bs, 128) positions
 // of one head, 128-byte swizzle, zeros outside (past hd, and in block `blocks`).
 bool make_map_pool(CUtensorMap *m, const void *pool, uint64_t blocks, uint64_t bs,
                    uint64_t kv_heads, uint64_t hd) {
@@ -1545,7 +1551,7 @@ bool make_map_pool(CUtensorMap *m, const void *pool, uint64_t blocks, uint64_t b
   if (!enc) return false;
   cuuint64_t dims[4] = {hd, bs, 2 * kv_heads, blocks};
   cuuint64_t strides[3] = {hd * 2, bs * hd * 2, 2 * kv_heads * bs * hd * 2};
-  cuuint32_t box[4] = {64, cuuint32_t(std::min<uint64_t>(bs, 64)), 1, 1};
+  cuuint32_t box[4] = {64, cuuint32_t(std::min<uint64_t>(bs, 128)), 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(pool), dims, strides, box,
              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1667,41 +1673,36 @@ wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, in
   a.words = mask ? int(mask_words) : 0;
   a.rows = int(rows);
   a.max_rows = int(max_rows);
-  a.max_len = int(max_len);
   a.heads = int(heads);
   a.kv_heads = int(kv_heads);
   a.hd = int(hd);
   a.scale = 1.0f / std::sqrt(float(hd));
-  // Positions past the tables' end are nobody's.
-  const uint64_t reach = std::min<uint64_t>(max_len, uint64_t(width) * bs);
-  const wv::AttendTreePlan plan = wv::attend_tree_plan(int(n), int(max_rows), int(reach),
-                                                       int(heads), int(kv_heads), ctx->sms);
-  a.splits = plan.splits;
-  a.chunk = plan.chunk;
+  a.max_len = int(std::min<uint64_t>(max_len, uint64_t(width) * bs));
+  a.n = int(n);
   a.err = ctx->dev_err;
-  if (plan.splits > 1) {
-    void *ws = nullptr;
-    const wavo_status got = workspace(
-        ctx, size_t(rows) * heads * plan.splits * (hd + 4) * sizeof(float), &ws);
-    if (got != WAVO_OK) return got;
-    a.part = static_cast<float *>(ws);
-  }
+  a.count = ctx->dev_err + kTreeCounts;
+  void *ws = nullptr;
+  const int f16 = dtype == WAVO_F16;
+  const wavo_status got = workspace(
+      ctx, wv::attend_tree_part_bytes(int(max_rows), int(heads), int(kv_heads), int(hd), f16, ctx->sms),
+      &ws);
+  if (got != WAVO_OK) return got;
+  a.part = static_cast<float *>(ws);
   CUtensorMap map;
   if (!make_map_pool(&map, pool, blocks, bs, kv_heads, hd))
     return fail(ctx, WAVO_ECUDA, "attend_tree: tensor map");
-  CK(wv::launch_attend_tree(map, a, plan, dtype == WAVO_F16, int(n), ctx->stream),
-     "attend_tree launch");
+  CK(wv::launch_attend_tree(map, a, f16, ctx->sms, ctx->stream), "attend_tree launch");
   return WAVO_OK;
 }
 
-size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t n, uint32_t rows, uint32_t max_rows,
-                                uint32_t max_len, uint32_t heads, uint32_t kv_heads, uint32_t hd) {
-  if (!ctx || !n || !rows || !max_rows || !kv_heads || heads < kv_heads || max_len > 0x7fffffffu)
-    return 0;
-  const wv::AttendTreePlan p =
-      wv::attend_tree_plan(int(n), int(std::min(max_rows, rows)), int(max_len), int(heads),
-                           int(kv_heads), ctx->sms);
-  return p.splits > 1 ? size_t(rows) * heads * p.splits * (hd + 4) * sizeof(float) : 0;
+size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t max_rows, uint32_t heads,
+                                uint32_t kv_heads, uint32_t hd) {
+  if (!ctx || !max_rows || !kv_heads || heads < kv_heads || max_rows > 0x7fffffffu) return 0;
+  size_t most = 0;
+  for (int f16 = 0; f16 < 2; ++f16)
+    most = std::max(most, wv::attend_tree_part_bytes(int(max_rows), int(heads), int(kv_heads),
+                                                     int(hd), f16, ctx->sms));
+  return most;
 }
 
 wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint64_t ld, void *out,
@@ -1716,7 +1717,7 @@ wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint
   if (ld == 0) ld = r->vocab;
   if (ld_out == 0) ld_out = r->vocab;
   if (r->vocab == 0 || r->vocab > 0x7fff0000u || ld < r->vocab || ld_out < r->vocab ||
-      (ld | ld_out) >> 31 || r->n == 0 || r->n > 0x7fffffffu || rows > 0x7fffffffu)
+      (ld | ld_out) >> 31 || r->n == 0 || r->n > 0x7fffffffu || rows > 65535)
     return fail(ctx, WAVO_EINVAL, "shape_logits: %u rows of %u tokens, strides %llu and %llu, %u "
                 "requests", rows, r->vocab, (unsigned long long)ld, (unsigned long long)ld_out, r->n);
   if (out == logits && ld_out != ld)
