@@ -260,7 +260,7 @@ struct ShapeArgs {
   int *picks;
   float *logprobs;
 };
-cudaError_t launch_shape(const ShapeArgs &a, int f16, cudaStream_t s);
+cudaError_t launch_shape(const ShapeArgs &a, int f16, int sms, cudaStream_t s);
 
 struct TreeAcceptArgs {
   const int *picks, *tokens;

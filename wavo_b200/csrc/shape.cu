@@ -8,18 +8,23 @@
 namespace wv {
 namespace {
 
-// A row's vocabulary is cut into slices, one a CTA; the CTAs of a row form a cluster (8 at most, and
-// a larger vocabulary goes round). A thread keeps SH_J of the slice's logits in registers: they are
-// read once, edited, written where they are wanted, and reduced to (maximum, its first index, sum of
-// exponentials) in one pass, which meets the other CTAs' through distributed shared memory.
-// What a row's tokens say of a slice stands in a word of shared memory a token: how often it is among
-// the history and the row's path in the low half, 1 + the last entry of its bias in the high half.
-// Counts and entries are whole numbers, so the order of the atomics does not matter. The logits are on
-// their way while the words are made.
+// A row's vocabulary is cut into ranges, one a CTA; the CTAs of a row form a cluster (8 at most). A
+// range passes through registers, four tokens a load and the next ones on their way: read once, masked,
+// written where it is wanted, and reduced to (maximum, its first index, sum of exponentials), which
+// meets the other CTAs' through distributed shared memory.
+// The tokens that a row's history, path or biases name are few, and their edits (a division among
+// them) many times the work of the others'. A bit a token takes them out of that pass; in the order of
+// their ids they have a place each in a list, with a word: how often the token is in the history and
+// the path in the low half, 1 + the last entry of its bias in the high half (whole numbers, so the
+// order of the atomics does not matter). A thread edits one of them.
 constexpr int SH_THREADS = 512;
-constexpr int SH_J = 16;                     // logits a thread holds
-constexpr int SH_SLICE = SH_THREADS * SH_J;  // logits a CTA holds at a time
-constexpr int SH_CTAS = 8;
+constexpr int SH_WARPS = SH_THREADS / 32;
+constexpr int SH_G = 2;                         // groups of four tokens a thread holds
+constexpr int SH_STEP = SH_THREADS * SH_G * 4;  // tokens a CTA holds at a time
+constexpr int SH_NAMED = 4096;                  // named tokens that the list holds
+constexpr int SH_SLICE = 65536;                 // tokens a range goes through at a time
+constexpr int SH_CTAS = 8;                      // of a cluster
+constexpr float SH_LOG2E = 1.4426950408889634f;
 
 struct ShapePart {
   float top, sum;  // the largest value, the sum of exp(value - top)
@@ -29,19 +34,52 @@ struct ShapePart {
 // Two parts as one: ties go to the lower index; a NaN sum stays.
 __device__ __forceinline__ void shape_join(ShapePart &a, float top, float sum, int at) {
   const float m = fmaxf(a.top, top), base = m == -INFINITY ? 0.0f : m;
-  a.sum = a.sum * __expf(a.top - base) + sum * __expf(top - base);
+  a.sum = a.sum * ex2((a.top - base) * SH_LOG2E) + sum * ex2((top - base) * SH_LOG2E);
   if (top > a.top || (top == a.top && at < a.at)) a.at = at;
   a.top = m;
 }
 
+template <int LANES>
+__device__ __forceinline__ void shape_join_lanes(ShapePart &a) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1)
+    shape_join(a, __shfl_xor_sync(0xffffffffu, a.top, o), __shfl_xor_sync(0xffffffffu, a.sum, o),
+               __shfl_xor_sync(0xffffffffu, a.at, o));
+}
+
+__device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
+  *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(p);
+}
+__device__ __forceinline__ void load4(const __half *p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2 *>(p);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+__device__ __forceinline__ void store4(float *p, const float (&x)[4]) {
+  *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void store4(__half *p, const float (&x)[4]) {
+  *reinterpret_cast<uint2 *>(p) = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+}
+
+struct ShapeShared {
+  uint32_t named[SH_SLICE / 32];    // a bit a place: a named token
+  uint16_t before[SH_SLICE / 32];   // the bits of the words before each
+  int list[SH_NAMED];               // the named tokens in order
+  uint32_t note[SH_NAMED];
+  int scan[SH_WARPS];
+  ShapePart warps[SH_WARPS], part;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(SH_THREADS, 2) shape_kernel(const ShapeArgs a, int slice) {
+__global__ void __launch_bounds__(SH_THREADS, 2)
+    shape_kernel(const ShapeArgs a, int range, int slice) {
   griddep_launch_dependents();
   griddep_wait();  // the previous kernel of the stream has completed (programmatic launch)
-  __shared__ alignas(16) uint32_t note[SH_SLICE];
-  __shared__ ShapePart warps[SH_THREADS / 32], part;
-  const int r = int(blockIdx.y), tid = int(threadIdx.x), lane = tid & 31, w = tid >> 5;
-  const int ctas = int(gridDim.x), rank = int(blockIdx.x);
+  __shared__ ShapeShared sh;
+  const int tid = int(threadIdx.x), lane = tid & 31, w = tid >> 5;
+  const int r = int(blockIdx.y), ctas = int(gridDim.x), rank = int(blockIdx.x);
   const int s = a.row_seq ? a.row_seq[r] : r;
   if (s < 0 || s >= a.n) {  // padding
     if (rank == 0 && tid == 0) {
@@ -52,113 +90,222 @@ __global__ void __launch_bounds__(SH_THREADS, 2) shape_kernel(const ShapeArgs a,
   }
   const T *in = static_cast<const T *>(a.logits) + r * a.ld;
   T *out = a.out ? static_cast<T *>(a.out) + r * a.ld_out : nullptr;
+  // Places are token + shift, so that a place that four divides is an aligned address.
+  const int shift = int(reinterpret_cast<uintptr_t>(in) / sizeof(T)) & 3;
+  const bool vec_out =
+      ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & (4 * sizeof(T) - 1)) == 0;
+  const int places = a.vocab + shift, last = (a.vocab - 1) >> 5;
+  const auto fetch = [&](int v, int hi, float (&x)[4]) {  // places v .. v + 3, -inf outside the row
+    const int i = v - shift;
+    if (v < hi && i >= 0 && i + 3 < a.vocab) {
+      load4(in + i, x);
+    } else {
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        x[y] = v < hi && i + y >= 0 && i + y < a.vocab ? float(in[i + y]) : -INFINITY;
+    }
+  };
+  const int begin = rank * range, end = min(begin + range, places);
+  float next[SH_G][4];
+#pragma unroll
+  for (int j = 0; j < SH_G; ++j)
+    fetch(begin + 4 * (tid + SH_THREADS * j), min(begin + slice, end), next[j]);
   const bool pen = a.penalties != nullptr;
-  const float rep = pen ? a.penalties[3 * s] : 1.0f, pres = pen ? a.penalties[3 * s + 1] : 0.0f,
-              freq = pen ? a.penalties[3 * s + 2] : 0.0f;
   const int hist = pen && a.history ? min(max(a.hist_len[s], 0), a.max_hist) : 0;
   const int path = pen && a.path ? a.path_words * 32 : 0;
   const int bias = a.bias_ids ? min(max(a.bias_len[s], 0), a.max_bias) : 0;
-  const int g = a.grammar ? a.grammar_of[r] : -1;
-  const uint32_t *allow = g >= 0 && g < a.n_grammar ? a.grammar + (long long)g * a.grammar_ld : nullptr;
+  const int set = a.grammar ? a.grammar_of[r] : -1;
+  const uint32_t *allow =
+      set >= 0 && set < a.n_grammar ? a.grammar + (long long)set * a.grammar_ld : nullptr;
   const int first_row = path ? a.row_start[s] : 0;
-  const bool notes = hist + path + bias > 0;
+  const int *history = a.history + (long long)s * a.max_hist;
+  const int *bias_ids = a.bias_ids + (long long)s * a.max_bias;
+  const bool any_named = hist + path + bias > 0;
+  // Drafted token i of the request if it is on the row's path, else -1.
+  const auto path_token = [&](int i) {
+    const int at = first_row + i;
+    return at >= 0 && at < a.rows &&
+                   ((a.path[(long long)r * a.path_words + (i >> 5)] >> (i & 31)) & 1u)
+               ? a.tokens[at]
+               : -1;
+  };
   ShapePart all = {-INFINITY, 0.0f, 0x7fffffff};
-  for (int lo = rank * slice; lo < a.vocab; lo += ctas * slice) {
-    const int cnt = min(slice, a.vocab - lo);
-    float x[SH_J];
-    uint32_t bits[SH_J];
-#pragma unroll
-    for (int j = 0; j < SH_J; ++j) {
-      const int i = tid + SH_THREADS * j;
-      x[j] = i < cnt ? float(in[lo + i]) : -INFINITY;
-      // Slices begin at multiples of 32: a warp's 32 tokens share a word.
-      bits[j] = allow && i < cnt ? allow[(lo + i) >> 5] : ~0u;
-    }
-    if (notes) {
-      for (int i = tid; i < SH_SLICE / 4; i += SH_THREADS)
-        reinterpret_cast<uint4 *>(note)[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (int lo = begin; lo < end; lo += slice) {
+    const int hi = min(lo + slice, end), words = (hi - lo + 31) / 32;
+    int listed = 0;
+    if (any_named) {
+      const unsigned cnt = unsigned(hi - lo);
+      const auto place = [&](int id) {  // the token's place in the slice, or past it
+        return id >= 0 && id < a.vocab ? unsigned(id + shift - lo) : ~0u;
+      };
+      // A thread's first entries stay in registers.
+      const int h0 = tid < hist ? history[tid] : -1, b0 = tid < bias ? bias_ids[tid] : -1;
+      const int p0 = tid < path ? path_token(tid) : -1;
+      for (int i = tid; i < words; i += SH_THREADS) sh.named[i] = 0u;
       __syncthreads();
-      if (bias > 0) {
-        for (int i = tid; i < bias; i += SH_THREADS) {
-          const unsigned id = unsigned(a.bias_ids[(long long)s * a.max_bias + i] - lo);
-          if (id < unsigned(cnt)) atomicMax(&note[id], uint32_t(i + 1) << 16);
+      const auto each = [&](const auto &use) {
+        use(place(h0), -1);
+        for (int i = tid + SH_THREADS; i < hist; i += SH_THREADS) use(place(history[i]), -1);
+        use(place(p0), -1);
+        for (int i = tid + SH_THREADS; i < path; i += SH_THREADS) use(place(path_token(i)), -1);
+      };
+      const auto each_bias = [&](const auto &use) {
+        use(place(b0), tid);
+        for (int i = tid + SH_THREADS; i < bias; i += SH_THREADS) use(place(bias_ids[i]), i);
+      };
+      const auto name = [&](unsigned to, int) {
+        if (to < cnt) atomicOr(&sh.named[to >> 5], 1u << (to & 31));
+      };
+      each(name);
+      each_bias(name);
+      __syncthreads();
+      // Where each word's tokens begin in the list: four words a thread.
+      int mine[4], sum = 0;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        mine[y] = sum;
+        if (4 * tid + y < words) sum += __popc(sh.named[4 * tid + y]);
+      }
+      int upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+      }
+      if (lane == 31) sh.scan[w] = upto;
+      __syncthreads();
+      int at = upto - sum;
+      for (int k = 0; k < SH_WARPS; ++k) {
+        if (k < w) at += sh.scan[k];
+        listed += sh.scan[k];
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        if (4 * tid + y < words) sh.before[4 * tid + y] = uint16_t(at + mine[y]);
+      for (int i = tid; i < listed; i += SH_THREADS) sh.note[i] = 0u;
+      __syncthreads();
+      const auto rank_of = [&](unsigned to) {
+        return int(sh.before[to >> 5]) + __popc(sh.named[to >> 5] & ((1u << (to & 31)) - 1u));
+      };
+      each_bias([&](unsigned to, int entry) {
+        if (to < cnt) {
+          const int k = rank_of(to);
+          sh.list[k] = int(to);
+          atomicMax(&sh.note[k], uint32_t(entry + 1) << 16);
         }
-        __syncthreads();  // the counts are added to the entries
-      }
-      for (int i = tid; i < hist; i += SH_THREADS) {
-        const unsigned id = unsigned(a.history[(long long)s * a.max_hist + i] - lo);
-        if (id < unsigned(cnt)) atomicAdd(&note[id], 1u);
-      }
-      for (int i = tid; i < path; i += SH_THREADS) {
-        const int at = first_row + i;
-        if (at < 0 || at >= a.rows ||
-            !((a.path[(long long)r * a.path_words + (i >> 5)] >> (i & 31)) & 1u))
-          continue;
-        const unsigned id = unsigned(a.tokens[at] - lo);
-        if (id < unsigned(cnt)) atomicAdd(&note[id], 1u);
-      }
+      });
+      if (bias > 0) __syncthreads();  // the counts are added to the entries
+      each([&](unsigned to, int) {
+        if (to < cnt) {
+          const int k = rank_of(to);
+          sh.list[k] = int(to);
+          atomicAdd(&sh.note[k], 1u);
+        }
+      });
       __syncthreads();
+      const float rep = pen ? a.penalties[3 * s] : 1.0f, pres = pen ? a.penalties[3 * s + 1] : 0.0f;
+      const float freq = pen ? a.penalties[3 * s + 2] : 0.0f;
+      for (int k = tid; k < listed; k += SH_THREADS) {
+        const int i = sh.list[k] + lo - shift;
+        const uint32_t e = sh.note[k], c = e & 0xffffu;
+        float z = float(in[i]);
+        if (c) {
+          z = z > 0.0f ? z / rep : z * rep;
+          z = __fsub_rn(z, __fadd_rn(__fmul_rn(freq, float(c)), pres));
+        }
+        if (e >> 16) z += a.bias_vals[(long long)s * a.max_bias + (e >> 16) - 1];
+        if (allow && !((allow[i >> 5] >> (i & 31)) & 1u)) z = -INFINITY;
+        sh.note[k] = __float_as_uint(z);
+        shape_join(all, z, z == -INFINITY ? 0.0f : isnan(z) ? z : 1.0f, i);
+      }
+      if (out == in) __syncthreads();  // the pass writes over what was read here
+    }
+#pragma unroll 1
+    for (int v0 = lo + 4 * tid; v0 - 4 * tid < hi; v0 += SH_STEP) {
+      float x[SH_G][4];
 #pragma unroll
-      for (int j = 0; j < SH_J; ++j) {
-        const int i = tid + SH_THREADS * j;
-        const uint32_t e = i < cnt ? note[i] : 0u;
-        if (e) {
-          const uint32_t c = e & 0xffffu;
-          float v = x[j];
-          if (c) {
-            v = v > 0.0f ? v / rep : v * rep;
-            v = __fsub_rn(v, __fadd_rn(__fmul_rn(freq, float(c)), pres));
+      for (int j = 0; j < SH_G; ++j) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[j][y] = next[j][y];
+        // The next step's, or the next slice's first.
+        const int v = v0 + SH_STEP + 4 * SH_THREADS * j;
+        const bool on = v0 - 4 * tid + SH_STEP < hi;
+        fetch(on ? v : hi + 4 * (tid + SH_THREADS * j), on ? hi : min(hi + slice, end), next[j]);
+      }
+      float top = all.top;
+#pragma unroll
+      for (int j = 0; j < SH_G; ++j) {
+        const int v = v0 + 4 * SH_THREADS * j, i = v - shift;
+        if (v < hi) {
+          const bool whole = i >= 0 && i + 3 < a.vocab;
+          // What the pass keeps of the four: allowed and not named (those come after).
+          uint32_t drop = 0u;
+          if (allow) {
+            const int i0 = max(i, 0), q = i0 >> 5;
+            drop = ~(__funnelshift_r(allow[q], allow[min(q + 1, last)], i0 & 31) << (i0 - i));
           }
-          if (e >> 16) v += a.bias_vals[(long long)s * a.max_bias + (e >> 16) - 1];
-          x[j] = v;
+          if (listed) drop |= sh.named[(v - lo) >> 5] >> ((v - lo) & 31);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) x[j][y] = drop & (1u << y) ? -INFINITY : x[j][y];
+          if (out) {
+            if (vec_out && whole) {
+              store4(out + i, x[j]);
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                if (i + y >= 0 && i + y < a.vocab) out[i + y] = T(x[j][y]);
+            }
+          }
+          if (fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])) > top) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (x[j][y] > top) {
+                top = x[j][y];
+                all.at = i + y;
+              }
+          }
         }
       }
-      if (lo + ctas * slice < a.vocab) __syncthreads();  // the words are made anew
-    }
-    ShapePart mine = {-INFINITY, 0.0f, 0x7fffffff};
-#pragma unroll
-    for (int j = 0; j < SH_J; ++j) {
-      const int i = tid + SH_THREADS * j;
-      if (!((bits[j] >> ((lo + i) & 31)) & 1u)) x[j] = -INFINITY;
-      if (out && i < cnt) out[lo + i] = T(x[j]);
-      if (x[j] > mine.top) {
-        mine.top = x[j];
-        mine.at = lo + i;
+      const float base = top == -INFINITY ? 0.0f : top * SH_LOG2E;
+      if (top > all.top) {
+        all.sum *= ex2(fmaf(all.top, SH_LOG2E, -base));
+        all.top = top;
       }
-    }
-    const float base = mine.top == -INFINITY ? 0.0f : mine.top;
 #pragma unroll
-    for (int j = 0; j < SH_J; ++j) mine.sum += __expf(x[j] - base);
-    shape_join(all, mine.top, mine.sum, mine.at);
+      for (int j = 0; j < SH_G; ++j)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) all.sum += ex2(fmaf(x[j][y], SH_LOG2E, -base));
+    }
+    if (listed) {
+      __syncthreads();  // the pass has written its values there
+      if (out)
+        for (int k = tid; k < listed; k += SH_THREADS)
+          out[sh.list[k] + lo - shift] = T(__uint_as_float(sh.note[k]));
+    }
+    if (any_named && hi < end) __syncthreads();  // the list is made anew
   }
   if (!a.picks && !a.logprobs) return;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    shape_join(all, __shfl_xor_sync(0xffffffffu, all.top, o), __shfl_xor_sync(0xffffffffu, all.sum, o),
-               __shfl_xor_sync(0xffffffffu, all.at, o));
-  if (lane == 0) warps[w] = all;
+  shape_join_lanes<32>(all);
+  if (lane == 0) sh.warps[w] = all;
   __syncthreads();
   if (w == 0) {
-    all = lane < SH_THREADS / 32 ? warps[lane] : ShapePart{-INFINITY, 0.0f, 0x7fffffff};
-#pragma unroll
-    for (int o = SH_THREADS / 64; o > 0; o >>= 1)
-      shape_join(all, __shfl_xor_sync(0xffffffffu, all.top, o),
-                 __shfl_xor_sync(0xffffffffu, all.sum, o), __shfl_xor_sync(0xffffffffu, all.at, o));
-    if (lane == 0) part = all;
+    all = sh.warps[lane % SH_WARPS];
+    shape_join_lanes<SH_WARPS>(all);
+    if (lane == 0) sh.part = all;
   }
   if (ctas > 1) cluster_sync();
   if (rank == 0 && tid == 0) {
     for (int p = 1; p < ctas; ++p) {
       uint32_t v[3];
 #pragma unroll
-      for (int k = 0; k < 3; ++k)
+      for (int x = 0; x < 3; ++x)
         asm volatile("ld.shared::cluster.u32 %0, [%1];"
-                     : "=r"(v[k])
-                     : "r"(mapa_shared(&part, p) + 4 * k)
+                     : "=r"(v[x])
+                     : "r"(mapa_shared(&sh.part, p) + 4 * x)
                      : "memory");
       shape_join(all, __uint_as_float(v[0]), __uint_as_float(v[1]), int(v[2]));
     }
-    const bool dead = all.top == -INFINITY;
+    const bool dead = all.top == -INFINITY;  // nothing left
     if (a.picks) a.picks[r] = dead ? -1 : all.at;
     if (a.logprobs) a.logprobs[r] = !dead ? -logf(all.sum) : isnan(all.sum) ? all.sum : -INFINITY;
   }
@@ -166,10 +313,18 @@ __global__ void __launch_bounds__(SH_THREADS, 2) shape_kernel(const ShapeArgs a,
 }
 
 template <typename T>
-cudaError_t launch(const ShapeArgs &a, cudaStream_t s) {
-  const int ctas = std::min(SH_CTAS, (a.vocab + SH_SLICE - 1) / SH_SLICE);
-  const int rounds = (a.vocab + ctas * SH_SLICE - 1) / (ctas * SH_SLICE);
-  const int slice = ((a.vocab + ctas * rounds - 1) / (ctas * rounds) + 31) / 32 * 32;
+cudaError_t launch(const ShapeArgs &a, int sms, cudaStream_t s) {
+  // As many CTAs a row (a power of two) as fill the SMs' two places each; ranges of 2048 tokens at
+  // least.
+  int ctas = 1;
+  while (ctas < SH_CTAS && a.rows * 1ll * ctas < 2ll * sms && a.vocab / (2 * ctas) >= 2048) ctas *= 2;
+  const int places = a.vocab + 3;
+  const int range = ((places + ctas - 1) / ctas + 31) / 32 * 32;
+  // The list holds every named token of a slice.
+  const long long named = (long long)(a.penalties && a.history ? a.max_hist : 0) +
+                          (a.penalties && a.path ? 32 * a.path_words : 0) +
+                          (a.bias_ids ? a.max_bias : 0);
+  const int slice = std::min(range, named <= SH_NAMED ? SH_SLICE : SH_NAMED);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, a.rows);
   cfg.blockDim = dim3(SH_THREADS);
@@ -183,14 +338,14 @@ cudaError_t launch(const ShapeArgs &a, cudaStream_t s) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, shape_kernel<T>, a, slice);
+  return cudaLaunchKernelEx(&cfg, shape_kernel<T>, a, range, slice);
 }
 
 }  // namespace
 
-cudaError_t launch_shape(const ShapeArgs &a, int f16, cudaStream_t s) {
+cudaError_t launch_shape(const ShapeArgs &a, int f16, int sms, cudaStream_t s) {
   if (a.rows <= 0) return cudaSuccess;
-  return f16 ? launch<__half>(a, s) : launch<float>(a, s);
+  return f16 ? launch<__half>(a, sms, s) : launch<float>(a, sms, s);
 }
 
 }  // namespace wv

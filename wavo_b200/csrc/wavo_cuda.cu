@@ -1766,7 +1766,7 @@ wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint
   a.path_words = int(r->path_words);
   a.picks = picks;
   a.logprobs = logprobs;
-  CK(wv::launch_shape(a, dtype == WAVO_F16, ctx->stream), "shape_logits launch");
+  CK(wv::launch_shape(a, dtype == WAVO_F16, ctx->sms, ctx->stream), "shape_logits launch");
   return WAVO_OK;
 }
 
