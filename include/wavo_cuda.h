@@ -394,8 +394,8 @@ wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, in
                              uint32_t n, const uint32_t *mask, uint32_t mask_words, uint32_t rows,
                              uint32_t max_rows, uint32_t max_len, void *o, uint64_t o_stride,
                              uint32_t heads, uint32_t kv_heads, uint32_t hd);
-size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t max_rows, uint32_t heads,
-                                uint32_t kv_heads, uint32_t hd);
+size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t n, uint32_t rows, uint32_t max_rows,
+                                uint32_t max_len, uint32_t heads, uint32_t kv_heads, uint32_t hd);
 
 /* What wavo_shape_logits applies to a row of a request, each part off where its pointers are NULL.
  * Device buffers; the struct itself is read at the call. */

@@ -114,7 +114,7 @@ SIGNATURES = {
     "wavo_pack_slots": ([_vp, _vp, _i32, _u32, _u32, _vp, _u32, _vp, _u32, _u32, _u32, _u32], _st),
     "wavo_attend_tree": ([_vp, _vp, _u64, _i32, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _u32, _vp,
                           _u32, _u32, _u32, _u32, _vp, _u64, _u32, _u32, _u32], _st),
-    "wavo_attend_tree_scratch": ([_vp, _u32, _u32, _u32, _u32], _sz),
+    "wavo_attend_tree_scratch": ([_vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32], _sz),
     "wavo_shape_logits": ([_vp, _vp, _i32, _u64, _vp, _u64, _u32, ctypes.POINTER(LogitRulesC),
                            _vp, _vp], _st),
     "wavo_tree_accept": ([_vp, _vp, _vp, _vp, _u32, _u32, _vp, _u32, _u32, _vp, _vp, _u32, _vp,

@@ -16,8 +16,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 SOURCES = ["wavo_cuda.cu", "gemm.cu", "attention.cu", "attention_fa.cu", "decode.cu", "selftest.cu",
-           "encoder.cu", "decoder.cu", "gguf.cu", "frontend.cu", "paged.cu", "tree.cu", "shape.cu"]
-HEADERS = ["ptx.cuh", "kernels.cuh", "softmax.cuh", "gguf.cuh"]
+           "encoder.cu", "decoder.cu", "gguf.cu", "frontend.cu", "paged.cu", "tree.cu", "tree_few.cu",
+           "shape.cu"]
+HEADERS = ["ptx.cuh", "kernels.cuh", "softmax.cuh", "gguf.cuh", "tree.cuh"]
 SO = os.path.join(HERE, "libwavo_cuda.so")
 STATIC = os.path.join(HERE, "libwavo_cuda.a")
 STAMP = os.path.join(HERE, ".libwavo_cuda.stamp")

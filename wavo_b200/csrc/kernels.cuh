@@ -225,11 +225,25 @@ struct AttendTreeArgs {
   int heads, kv_heads, hd;
   float scale;           // 1 / sqrt(hd)
   int n;                 // requests
-  float *part;           // parts of items that span several runs (attend_tree_part_bytes)
-  int *count;            // parts written of each, kTreeRunsPerSm a SM, 0 between launches
+  int splits, chunk;     // few rows: ranges of `chunk` positions, one CTA each
+  float *part;           // parts of items that span several CTAs
+  int *count;            // many rows: parts written of each, kTreeRunsPerSm a SM, 0 between launches
   int *err;              // device error word
 };
+// Few rows (tree_few.cu): every request, K and V head and 64 rows has `splits` CTAs, over `chunk`
+// positions each. map: as below, boxes of min(bs, 64) positions.
+struct AttendFewPlan {
+  int splits, chunk;
+};
+AttendFewPlan attend_few_plan(int n, int max_rows, int max_len, int heads, int kv_heads, int hd,
+                              int sms);
+size_t attend_few_part_bytes(const AttendFewPlan &p, int rows, int heads, int hd);
+cudaError_t launch_attend_few(const CUtensorMap &map, const AttendTreeArgs &a, int f16,
+                              cudaStream_t s);
+// Many rows (tree.cu).
 constexpr int kTreeRunsPerSm = 2;
+// Whether a call goes to the few-rows kernel.
+bool attend_tree_few(int max_rows, int heads, int kv_heads, int f16);
 // Rows of an item: the rows of a request that read one K and V head, in steps that the kernel has.
 int attend_tree_rows(int max_rows, int heads, int kv_heads, int f16);
 size_t attend_tree_part_bytes(int max_rows, int heads, int kv_heads, int hd, int f16, int sms);

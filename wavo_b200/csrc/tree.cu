@@ -22,8 +22,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "kernels.cuh"
-#include "ptx.cuh"
+#include "tree.cuh"
 
 namespace wv {
 namespace {
@@ -33,29 +32,6 @@ constexpr uint32_t TT_HALF = TT_KEYS * 128;   // bytes of 128 positions x 64 ele
 constexpr float TT_RISE = 8.0f;
 constexpr int TT_PIECES = 3;                  // items in flight: loaded, multiplied, written
 constexpr int TT_WHOLE = 4;                   // items of up to this many tiles stay in one run
-
-__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar,
-                                            int x, int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
-
-// hi + lo = (x, y) to 2^-22 of each.
-__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
-  hi = pack_half2(x, y);
-  const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&hi));
-  lo = pack_half2(x - f.x, y - f.y);
-}
-
-// The pair with zeros for infinities and NaN.
-__device__ __forceinline__ uint32_t finite2(uint32_t v) {
-  if ((v & 0x7c00u) == 0x7c00u) v &= 0xffff0000u;
-  if ((v & 0x7c000000u) == 0x7c000000u) v &= 0x0000ffffu;
-  return v;
-}
 
 // v[k] of 32 lanes reduced for each k: lane k gets the result of v[k] (31 shuffles for 32 values; the
 // halves that a lane gives away it reads from its partner).
@@ -87,9 +63,9 @@ struct TreeTile {
   static constexpr int kPBufs = kCtas * kParts * kP >= 2 * TT_HALF ? 1 : 2;
   static constexpr int kQBufs = kParts * kQ > 16384 ? 1 : 2;
   static constexpr int kRing = HDP == 128 ? (kParts * NR >= 128 ? 3 : 4) : kCtas == 2 ? 4 : 8;
-  // Softmax warps: a group of four holds the 128 positions; two groups halve the rows.
-  static constexpr int kGroups = NR <= 32 ? 1 : 2;
-  static constexpr int kRows = NR / kGroups;                        // rows a thread holds
+  // Softmax warps: a group of four holds the 128 positions; the groups share the rows, 16 at a time.
+  static constexpr int kGroups = NR <= 32 ? 1 : 4;
+  static constexpr int kRows = NR / kGroups;                        // rows a thread holds at most
   static constexpr int kSoft = 128 * kGroups;
   static constexpr int kThreads = kSoft + 96;                       // and loads, UMMAs, rows
   static constexpr uint32_t kOffQ = kRing * kSlot;
@@ -121,7 +97,7 @@ struct TreeShared {
   TreeRows<NR> rows[TT_PIECES];
   uint32_t tmem, abort, last;
   uint32_t odd[8];              // drafted positions whose V holds an infinity or NaN
-  long long scan[12], begin, end;
+  long long scan[20], begin, end;
   int begin_s, begin_n;         // the run's first request and the tiles of it that lie before
   alignas(16) float lim[NR];    // a score above it raises its row's reference
   alignas(16) float base[NR];   // the reference (0 where a row has seen nothing)
@@ -447,42 +423,57 @@ __global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HD
           !mbar_wait_warp(&sh.q_empty[qb], (k / T::kQBufs - 1) & 1, ab, kErrTimeoutConsumer))
         break;
       uint8_t *base = smem + T::kOffQ + qb * T::kParts * T::kQ;
-      // Eight elements a lane and step, four steps in flight; rows to the next 16 are zeros.
+      // Eight elements a lane and step; rows to the next 16 are zeros.
       const int chunks = (q.here + 15) / 16 * 16 * (HDP / 8);
-      for (int e0 = lane; e0 < chunks; e0 += 128) {
-        E v[4][8];
+      const auto source = [&](int e) -> const E * {
+        const int r = e / (HDP / 8), c = e % (HDP / 8);
+        const int i = (q.r0 + r) / group, head = q.kvh * group + (q.r0 + r) - i * group;
+        if (e >= chunks || r >= q.here || q.lo + i >= a.rows || c * 8 >= a.hd) return nullptr;
+        return static_cast<const E *>(a.q) + (long long)(q.lo + i) * a.q_stride + head * a.hd + c * 8;
+      };
+      const auto target = [&](int e) {
+        const int r = e / (HDP / 8), c = e % (HDP / 8);
+        return base + (c >> 3) * NR * 128 + sw128_offset(r, c & 7);
+      };
+      if (!WIDE && vec) {
+        // As they are, all in flight at once.
+        for (int e = lane; e < chunks; e += 32) {
+          const E *from = source(e);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(target(e))),
+                       "l"(from ? from : static_cast<const E *>(a.q)), "r"(from ? 16 : 0)
+                       : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      } else {
+        for (int e0 = lane; e0 < chunks; e0 += 128) {  // four steps in flight
+          E v[4][8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int e = e0 + 32 * u, r = e / (HDP / 8), c = e % (HDP / 8);
-          const int i = (q.r0 + r) / group, head = q.kvh * group + (q.r0 + r) - i * group;
+          for (int u = 0; u < 4; ++u) {
+            const E *from = source(e0 + 32 * u);
 #pragma unroll
-          for (int x = 0; x < 8; ++x) v[u][x] = E(0.0f);
-          if (e < chunks && r < q.here && q.lo + i < a.rows && c * 8 < a.hd) {
-            const E *from = static_cast<const E *>(a.q) + (long long)(q.lo + i) * a.q_stride +
-                            head * a.hd + c * 8;
-            if (vec) {
+            for (int x = 0; x < 8; ++x) v[u][x] = E(0.0f);
+            if (from && vec) {
 #pragma unroll
               for (int x = 0; x < int(sizeof(E)) / 2; ++x)
                 reinterpret_cast<uint4 *>(v[u])[x] = reinterpret_cast<const uint4 *>(from)[x];
-            } else {
+            } else if (from) {
 #pragma unroll
               for (int x = 0; x < 8; ++x) v[u][x] = from[x];
             }
           }
-        }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int e = e0 + 32 * u, r = e / (HDP / 8), c = e % (HDP / 8);
-          if (e >= chunks) break;
-          uint8_t *at = base + (c >> 3) * NR * 128 + sw128_offset(r, c & 7);
-          if constexpr (WIDE) {
-            uint32_t hi[4], low[4];
+          for (int u = 0; u < 4; ++u) {
+            if (e0 + 32 * u >= chunks) break;
+            uint8_t *at = target(e0 + 32 * u);
+            if constexpr (WIDE) {
+              uint32_t hi[4], low[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) split2(v[u][2 * x], v[u][2 * x + 1], hi[x], low[x]);
-            *reinterpret_cast<uint4 *>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4 *>(at + T::kQ) = make_uint4(low[0], low[1], low[2], low[3]);
-          } else {
-            *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(v[u]);
+              for (int x = 0; x < 4; ++x) split2(v[u][2 * x], v[u][2 * x + 1], hi[x], low[x]);
+              *reinterpret_cast<uint4 *>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              *reinterpret_cast<uint4 *>(at + T::kQ) = make_uint4(low[0], low[1], low[2], low[3]);
+            } else {
+              *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(v[u]);
+            }
           }
         }
       }
@@ -508,8 +499,7 @@ __global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HD
           : "memory");
       return r != 0;
     };
-    const int key = tid & 127, quarter = w & 3, col0 = (w >> 2) * R;
-    const uint32_t lanes = tmem + (uint32_t(quarter) * 32u << 16) + col0;
+    const int key = tid & 127, quarter = w & 3;
     const float scale = a.scale * 1.4426950408889634f;  // exponentials of base 2
     int pv = 0;  // V's place in the ring
     for (int k = 0, g = 0; g < n; ++k) {
@@ -520,7 +510,11 @@ __global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HD
       if (any(!ok)) break;
       const TreePiece &q = sh.piece[pc];
       const TreeRows<NR> &rows = sh.rows[pc];
-      const int here = q.here, tiles = q.tiles;
+      // This group's rows: col0 up to `here`, an even share in steps of 16.
+      const int share = ((q.here + 15) / 16 + T::kGroups - 1) / T::kGroups * 16;
+      const int col0 = (w >> 2) * share, tiles = q.tiles;
+      const int here = min(q.here, col0 + share);
+      const uint32_t lanes = tmem + (uint32_t(quarter) * 32u << 16) + col0;
       const int *table = a.table + (long long)q.s * a.width;
       for (int r = tid; r < NR; r += SOFT) {
         sh.ref[r] = -INFINITY;
@@ -549,7 +543,8 @@ __global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HD
               if (d < 32 * a.words)
 #pragma unroll
                 for (int r = 0; r < (R < 32 ? R : 32); ++r)
-                  vis[x] |= ((rows.mask[col0 + 32 * x + r][d >> 5] >> (d & 31)) & 1u) << r;
+                  if (col0 + 32 * x + r < here)
+                    vis[x] |= ((rows.mask[col0 + 32 * x + r][d >> 5] >> (d & 31)) & 1u) << r;
             }
           }
         }
@@ -593,10 +588,11 @@ __global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HD
                 x[y] = r < R && col0 + r / 16 * 16 < here ? x_of(r % R) : -INFINITY;
               }
               const float top = lanes_reduce<true>(x);
-              if (32 * c + lane < R) sh.red[quarter][col0 + 32 * c + lane] = top;
+              if (32 * c + lane < R && col0 + 32 * c + lane < here)
+                sh.red[quarter][col0 + 32 * c + lane] = top;
             }
           sync();
-          for (int r = tid; r < here; r += SOFT) {
+          for (int r = tid; r < q.here; r += SOFT) {
             const float old = sh.ref[r];
             const float top =
                 fmaxf(fmaxf(sh.red[0][r], sh.red[1][r]), fmaxf(sh.red[2][r], sh.red[3][r]));
@@ -674,7 +670,7 @@ __global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HD
         // end, and a drafted position's infinities and NaN are zeros here and added at the end to the
         // rows that see them.
         pv = g == n - 1 ? 2 * n - 1 : 2 * g + 2;
-        if (!all && col0 == 0) {
+        if (!all && w < 4) {
           mbar_wait_warp(&sh.full[pv % D], (pv / D) & 1, ab, kErrTimeoutConsumer);
           uint8_t *v = smem + (pv % D) * T::kSlot;
           if (!there || d >= 0) {
@@ -706,10 +702,11 @@ __global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HD
 #pragma unroll
         for (int y = 0; y < 32; ++y) x[y] = 32 * c + y < R ? l[(32 * c + y) % R] : 0.0f;
         const float sum = lanes_reduce<false>(x);
-        if (32 * c + lane < R) sh.red[quarter][col0 + 32 * c + lane] = sum;
+        if (32 * c + lane < R && col0 + 32 * c + lane < here)
+          sh.red[quarter][col0 + 32 * c + lane] = sum;
       }
       sync();
-      for (int r = tid; r < NR; r += SOFT) {
+      for (int r = tid; r < q.here; r += SOFT) {
         const float sum = sh.red[0][r] + sh.red[1][r] + sh.red[2][r] + sh.red[3][r];
         sh.fac[r] = q.slot >= 0 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
         if (q.slot >= 0 && rows.out[r] >= 0)
@@ -769,7 +766,7 @@ __global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HD
             const long long slot = 2ll * (q.first + x) + (x == 0 ? 1 : 0);
             return a.part + (slot * NR + r) * (a.hd + 4);
           };
-          for (int r = tid; r < here; r += SOFT) {
+          for (int r = tid; r < q.here; r += SOFT) {
             float top = -INFINITY, sum = 0.0f;
             for (int x = 0; x < q.parts; ++x) top = fmaxf(top, __ldcg(part_of(x, r) + a.hd));
             const float base = top == -INFINITY ? 0.0f : top;
@@ -782,7 +779,7 @@ __global__ void __launch_bounds__(TreeTile<HDP, NR, WIDE>::kThreads, TreeTile<HD
           }
           sync();
           const int quads = a.hd / 4;
-          for (int e = tid; e < here * quads; e += SOFT) {
+          for (int e = tid; e < q.here * quads; e += SOFT) {
             const int r = e / quads, c = (e - r * quads) * 4;
             const int row = q.lo + (q.r0 + r) / group, head = q.kvh * group + (q.r0 + r) % group;
             if (row >= a.rows) continue;
@@ -856,6 +853,10 @@ cudaError_t launch_rows(const CUtensorMap &map, const AttendTreeArgs &a, int f16
 }
 
 }  // namespace
+
+bool attend_tree_few(int max_rows, int heads, int kv_heads, int f16) {
+  return (long long)max_rows * (heads / kv_heads) <= 64;
+}
 
 int attend_tree_rows(int max_rows, int heads, int kv_heads, int f16) {
   const long long rows = (long long)max_rows * (heads / kv_heads);

@@ -1543,15 +1543,15 @@ wavo_status wavo_attend(wavo_ctx *ctx, const float *q, const void *kv, float *pa
 
 namespace {
 
-// A paged cache as {hd, bs, 2 kv_heads, blocks} of f16, boxes of 64 elements x min(bs, 128) positions
+// A paged cache as {hd, bs, 2 kv_heads, blocks} of f16, boxes of 64 elements x min(bs, most) positions
 // of one head, 128-byte swizzle, zeros outside (past hd, and in block `blocks`).
 bool make_map_pool(CUtensorMap *m, const void *pool, uint64_t blocks, uint64_t bs,
-                   uint64_t kv_heads, uint64_t hd) {
+                   uint64_t kv_heads, uint64_t hd, uint64_t most) {
   EncodeTiled enc = encoder();
   if (!enc) return false;
   cuuint64_t dims[4] = {hd, bs, 2 * kv_heads, blocks};
   cuuint64_t strides[3] = {hd * 2, bs * hd * 2, 2 * kv_heads * bs * hd * 2};
-  cuuint32_t box[4] = {64, cuuint32_t(std::min<uint64_t>(bs, 128)), 1, 1};
+  cuuint32_t box[4] = {64, cuuint32_t(std::min(bs, most)), 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(pool), dims, strides, box,
              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1680,28 +1680,51 @@ wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, in
   a.max_len = int(std::min<uint64_t>(max_len, uint64_t(width) * bs));
   a.n = int(n);
   a.err = ctx->dev_err;
-  a.count = ctx->dev_err + kTreeCounts;
-  void *ws = nullptr;
   const int f16 = dtype == WAVO_F16;
-  const wavo_status got = workspace(
-      ctx, wv::attend_tree_part_bytes(int(max_rows), int(heads), int(kv_heads), int(hd), f16, ctx->sms),
-      &ws);
-  if (got != WAVO_OK) return got;
+  const bool few = wv::attend_tree_few(int(max_rows), int(heads), int(kv_heads), f16);
+  size_t bytes;
+  if (few) {
+    const wv::AttendFewPlan plan = wv::attend_few_plan(int(n), int(max_rows), a.max_len, int(heads),
+                                                       int(kv_heads), int(hd), ctx->sms);
+    a.splits = plan.splits;
+    a.chunk = plan.chunk;
+    bytes = wv::attend_few_part_bytes(plan, int(rows), int(heads), int(hd));
+  } else {
+    a.count = ctx->dev_err + kTreeCounts;
+    bytes = wv::attend_tree_part_bytes(int(max_rows), int(heads), int(kv_heads), int(hd), f16, ctx->sms);
+  }
+  void *ws = nullptr;
+  if (bytes) {
+    const wavo_status got = workspace(ctx, bytes, &ws);
+    if (got != WAVO_OK) return got;
+  }
   a.part = static_cast<float *>(ws);
   CUtensorMap map;
-  if (!make_map_pool(&map, pool, blocks, bs, kv_heads, hd))
+  if (!make_map_pool(&map, pool, blocks, bs, kv_heads, hd, few ? 64 : 128))
     return fail(ctx, WAVO_ECUDA, "attend_tree: tensor map");
-  CK(wv::launch_attend_tree(map, a, f16, ctx->sms, ctx->stream), "attend_tree launch");
+  CK(few ? wv::launch_attend_few(map, a, f16, ctx->stream)
+         : wv::launch_attend_tree(map, a, f16, ctx->sms, ctx->stream),
+     "attend_tree launch");
   return WAVO_OK;
 }
 
-size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t max_rows, uint32_t heads,
-                                uint32_t kv_heads, uint32_t hd) {
-  if (!ctx || !max_rows || !kv_heads || heads < kv_heads || max_rows > 0x7fffffffu) return 0;
+size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t n, uint32_t rows, uint32_t max_rows,
+                                uint32_t max_len, uint32_t heads, uint32_t kv_heads, uint32_t hd) {
+  if (!ctx || !n || !rows || !max_rows || !kv_heads || heads < kv_heads || max_rows > 0x7fffffffu ||
+      max_len > 0x7fffffffu || n > 65535)
+    return 0;
   size_t most = 0;
-  for (int f16 = 0; f16 < 2; ++f16)
-    most = std::max(most, wv::attend_tree_part_bytes(int(max_rows), int(heads), int(kv_heads),
-                                                     int(hd), f16, ctx->sms));
+  for (int f16 = 0; f16 < 2; ++f16) {
+    if (wv::attend_tree_few(int(max_rows), int(heads), int(kv_heads), f16)) {
+      // The ranges of a call follow from the positions that its tables reach, max_len at most.
+      const wv::AttendFewPlan plan = wv::attend_few_plan(int(n), int(max_rows), int(max_len),
+                                                         int(heads), int(kv_heads), int(hd), ctx->sms);
+      most = std::max(most, wv::attend_few_part_bytes(plan, int(rows), int(heads), int(hd)));
+    } else {
+      most = std::max(most, wv::attend_tree_part_bytes(int(max_rows), int(heads), int(kv_heads),
+                                                       int(hd), f16, ctx->sms));
+    }
+  }
   return most;
 }
 
