@@ -208,6 +208,11 @@ cudaError_t launch_pack_slots(const void *x, int x_f16, long long stride, const 
                               int rows, __half *pool, int nslots, int bs, int kv_heads, int hd,
                               int sms, cudaStream_t s);
 
+// Many rows (tree.cu): the item that a run begins and does not end, and the runs that it takes.
+struct TreeJoin {
+  int lo, r0, here, kvh, parts;
+};
+
 struct AttendTreeArgs {
   const void *q;
   long long q_stride;    // elements between rows
@@ -227,7 +232,7 @@ struct AttendTreeArgs {
   int n;                 // requests
   int splits, chunk;     // few rows: ranges of `chunk` positions, one CTA each
   float *part;           // parts of items that span several CTAs
-  int *count;            // many rows: parts written of each, kTreeRunsPerSm a SM, 0 between launches
+  TreeJoin *joins;       // many rows: one a run
   int *err;              // device error word
 };
 // Few rows (tree_few.cu): every request, K and V head and 64 rows has `splits` CTAs, over `chunk`
@@ -241,12 +246,9 @@ size_t attend_few_part_bytes(const AttendFewPlan &p, int rows, int heads, int hd
 cudaError_t launch_attend_few(const CUtensorMap &map, const AttendTreeArgs &a, int f16,
                               cudaStream_t s);
 // Many rows (tree.cu).
-constexpr int kTreeRunsPerSm = 2;
 // Whether a call goes to the few-rows kernel.
-bool attend_tree_few(int max_rows, int heads, int kv_heads, int f16);
-// Rows of an item: the rows of a request that read one K and V head, in steps that the kernel has.
-int attend_tree_rows(int max_rows, int heads, int kv_heads, int f16);
-size_t attend_tree_part_bytes(int max_rows, int heads, int kv_heads, int hd, int f16, int sms);
+bool attend_tree_few(int max_rows, int heads, int kv_heads, int hd);
+size_t attend_tree_part_bytes(int hd, int sms);
 // map: the pool as a 4D f16 tensor {hd, bs, 2 kv_heads, blocks}, boxes {64, min(bs, 128), 1, 1},
 // 128-byte swizzle, zeros outside.
 cudaError_t launch_attend_tree(const CUtensorMap &map, const AttendTreeArgs &a, int f16, int sms,

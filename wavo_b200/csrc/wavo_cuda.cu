@@ -27,7 +27,7 @@ struct wavo_ctx {
   int sms = 0;
   cudaStream_t own = nullptr;
   cudaStream_t stream = nullptr;
-  int *dev_err = nullptr;    // the kernels' error word, then attend_tree's counts (kTreeCounts on)
+  int *dev_err = nullptr;    // the kernels' error word
   void *ws = nullptr;        // scratch for casts and repacks
   size_t ws_bytes = 0;
   bool capturing = false;
@@ -279,12 +279,6 @@ wavo_status workspace(wavo_ctx *ctx, size_t bytes, void **out) {
   return WAVO_OK;
 }
 
-// The error word has a cache line of its own; the counts follow.
-constexpr int kTreeCounts = 32;
-size_t dev_words_bytes(const wavo_ctx *ctx) {
-  return (kTreeCounts + size_t(wv::kTreeRunsPerSm) * ctx->sms) * sizeof(int);
-}
-
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // IEEE binary16 from f32, round to nearest even (the reference GPU GEMM's rounding of W).
@@ -339,8 +333,8 @@ wavo_status wavo_create(int device, wavo_ctx **out) {
   ctx->sms = prop.multiProcessorCount;
   if ((e = cudaSetDevice(device)) != cudaSuccess ||
       (e = cudaStreamCreateWithFlags(&ctx->own, cudaStreamNonBlocking)) != cudaSuccess ||
-      (e = cudaMalloc(&ctx->dev_err, dev_words_bytes(ctx))) != cudaSuccess ||
-      (e = cudaMemset(ctx->dev_err, 0, dev_words_bytes(ctx))) != cudaSuccess) {
+      (e = cudaMalloc(&ctx->dev_err, sizeof(int))) != cudaSuccess ||
+      (e = cudaMemset(ctx->dev_err, 0, sizeof(int))) != cudaSuccess) {
     fail(nullptr, WAVO_ECUDA, "context setup: %s", cudaGetErrorString(e));
     if (ctx->own) cudaStreamDestroy(ctx->own);
     if (ctx->dev_err) cudaFree(ctx->dev_err);
@@ -449,7 +443,7 @@ wavo_status wavo_sync(wavo_ctx *ctx, uint32_t timeout_ms) {
   int code = 0;
   CK(cudaMemcpy(&code, ctx->dev_err, sizeof code, cudaMemcpyDeviceToHost), "error word");
   if (code) {
-    CK(cudaMemset(ctx->dev_err, 0, dev_words_bytes(ctx)), "error word reset");
+    CK(cudaMemset(ctx->dev_err, 0, sizeof(int)), "error word reset");
     static const char *what[] = {"", "TMA producer", "MMA issuer", "softmax/epilogue", "drain"};
     return fail(ctx, WAVO_EDEVICE, "a kernel's bounded wait gave up (%s, code %d)",
                 code > 0 && code < 5 ? what[code] : "?", code);
@@ -1681,7 +1675,7 @@ wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, in
   a.n = int(n);
   a.err = ctx->dev_err;
   const int f16 = dtype == WAVO_F16;
-  const bool few = wv::attend_tree_few(int(max_rows), int(heads), int(kv_heads), f16);
+  const bool few = wv::attend_tree_few(int(max_rows), int(heads), int(kv_heads), int(hd));
   size_t bytes;
   if (few) {
     const wv::AttendFewPlan plan = wv::attend_few_plan(int(n), int(max_rows), a.max_len, int(heads),
@@ -1690,8 +1684,7 @@ wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, in
     a.chunk = plan.chunk;
     bytes = wv::attend_few_part_bytes(plan, int(rows), int(heads), int(hd));
   } else {
-    a.count = ctx->dev_err + kTreeCounts;
-    bytes = wv::attend_tree_part_bytes(int(max_rows), int(heads), int(kv_heads), int(hd), f16, ctx->sms);
+    bytes = wv::attend_tree_part_bytes(int(hd), ctx->sms);
   }
   void *ws = nullptr;
   if (bytes) {
@@ -1699,6 +1692,9 @@ wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, in
     if (got != WAVO_OK) return got;
   }
   a.part = static_cast<float *>(ws);
+  if (!few)
+    a.joins = reinterpret_cast<wv::TreeJoin *>(static_cast<char *>(ws) + bytes -
+                                               ctx->sms * sizeof(wv::TreeJoin));
   CUtensorMap map;
   if (!make_map_pool(&map, pool, blocks, bs, kv_heads, hd, few ? 64 : 128))
     return fail(ctx, WAVO_ECUDA, "attend_tree: tensor map");
@@ -1713,19 +1709,12 @@ size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t n, uint32_t rows, 
   if (!ctx || !n || !rows || !max_rows || !kv_heads || heads < kv_heads || max_rows > 0x7fffffffu ||
       max_len > 0x7fffffffu || n > 65535)
     return 0;
-  size_t most = 0;
-  for (int f16 = 0; f16 < 2; ++f16) {
-    if (wv::attend_tree_few(int(max_rows), int(heads), int(kv_heads), f16)) {
-      // The ranges of a call follow from the positions that its tables reach, max_len at most.
-      const wv::AttendFewPlan plan = wv::attend_few_plan(int(n), int(max_rows), int(max_len),
-                                                         int(heads), int(kv_heads), int(hd), ctx->sms);
-      most = std::max(most, wv::attend_few_part_bytes(plan, int(rows), int(heads), int(hd)));
-    } else {
-      most = std::max(most, wv::attend_tree_part_bytes(int(max_rows), int(heads), int(kv_heads),
-                                                       int(hd), f16, ctx->sms));
-    }
-  }
-  return most;
+  if (!wv::attend_tree_few(int(max_rows), int(heads), int(kv_heads), int(hd)))
+    return wv::attend_tree_part_bytes(int(hd), ctx->sms);
+  // The ranges of a call follow from the positions that its tables reach, max_len at most.
+  return wv::attend_few_part_bytes(wv::attend_few_plan(int(n), int(max_rows), int(max_len),
+                                                       int(heads), int(kv_heads), int(hd), ctx->sms),
+                                   int(rows), int(heads), int(hd));
 }
 
 wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint64_t ld, void *out,
