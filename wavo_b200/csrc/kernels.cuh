@@ -247,7 +247,7 @@ cudaError_t launch_attend_few(const CUtensorMap &map, const AttendTreeArgs &a, i
                               cudaStream_t s);
 // Many rows (tree.cu).
 // Whether a call goes to the few-rows kernel.
-bool attend_tree_few(int max_rows, int heads, int kv_heads, int hd);
+bool attend_tree_few(int max_rows, int max_len, int heads, int kv_heads, int hd);
 size_t attend_tree_part_bytes(int hd, int sms);
 // map: the pool as a 4D f16 tensor {hd, bs, 2 kv_heads, blocks}, boxes {64, min(bs, 128), 1, 1},
 // 128-byte swizzle, zeros outside.

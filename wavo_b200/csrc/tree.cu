@@ -770,8 +770,15 @@ cudaError_t launch_tile(const CUtensorMap &map, const AttendTreeArgs &a, int sms
 
 }  // namespace
 
-bool attend_tree_few(int max_rows, int heads, int kv_heads, int hd) {
-  return (long long)max_rows * (heads / kv_heads) <= 64;
+// Measured on both sides (us, f16 / f32, few : many; 2 x 16384 positions unless said otherwise):
+// heads of 128: 24 rows 33 : 34 / 45 : 42, 48 rows 57 : 40 / 84 : 53, 96 rows 81 : 53 / 119 : 74;
+// heads of 64: 24 rows 37 : 50 / 49 : 59, 48 rows 56 : 58 / 83 : 65, 96 rows 84 : 56 / 143 : 83, but over 16 x 1024
+// positions 96 rows 57 : 66 / 70 : 81, and 128 rows of 32 x 512 103 : 135 (f32).
+bool attend_tree_few(int max_rows, int max_len, int heads, int kv_heads, int hd) {
+  const long long rows = (long long)max_rows * (heads / kv_heads);
+  if (rows <= 32) return true;
+  if (hd > 64 || rows > 128) return false;
+  return max_len < (rows > 64 ? 1280 : 2048);
 }
 
 size_t attend_tree_part_bytes(int hd, int sms) {

@@ -1675,7 +1675,8 @@ wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, in
   a.n = int(n);
   a.err = ctx->dev_err;
   const int f16 = dtype == WAVO_F16;
-  const bool few = wv::attend_tree_few(int(max_rows), int(heads), int(kv_heads), int(hd));
+  const bool few =
+      wv::attend_tree_few(int(max_rows), a.max_len, int(heads), int(kv_heads), int(hd));
   size_t bytes;
   if (few) {
     const wv::AttendFewPlan plan = wv::attend_few_plan(int(n), int(max_rows), a.max_len, int(heads),
@@ -1709,12 +1710,13 @@ size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t n, uint32_t rows, 
   if (!ctx || !n || !rows || !max_rows || !kv_heads || heads < kv_heads || max_rows > 0x7fffffffu ||
       max_len > 0x7fffffffu || n > 65535)
     return 0;
-  if (!wv::attend_tree_few(int(max_rows), int(heads), int(kv_heads), int(hd)))
-    return wv::attend_tree_part_bytes(int(hd), ctx->sms);
-  // The ranges of a call follow from the positions that its tables reach, max_len at most.
-  return wv::attend_few_part_bytes(wv::attend_few_plan(int(n), int(max_rows), int(max_len),
-                                                       int(heads), int(kv_heads), int(hd), ctx->sms),
-                                   int(rows), int(heads), int(hd));
+  // Of both kernels: which one a call takes, and its ranges, follow from the positions that its
+  // tables reach, max_len at most.
+  return std::max(wv::attend_tree_part_bytes(int(hd), ctx->sms),
+                  wv::attend_few_part_bytes(
+                      wv::attend_few_plan(int(n), int(max_rows), int(max_len), int(heads),
+                                          int(kv_heads), int(hd), ctx->sms),
+                      int(rows), int(heads), int(hd)));
 }
 
 wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint64_t ld, void *out,

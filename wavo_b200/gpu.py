@@ -35,26 +35,31 @@ def _dtype(t: torch.Tensor) -> int:
     raise TypeError(f"unsupported buffer dtype {t.dtype} (float32 or float16)")
 
 
-def _contiguous_ptr(t: torch.Tensor) -> int:
-    if not t.is_contiguous():
-        raise ValueError("buffers are contiguous")
-    return _ptr(t)
+_I32, _F32, _F16 = torch.int32, torch.float32, torch.float16
 
 
-def _int32(*tensors) -> None:
-    """Contiguous int32 buffers (None: left out)."""
-    for t in tensors:
-        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
-            raise TypeError("contiguous int32 buffers")
+def _i32(t) -> int:
+    """The address of a contiguous int32 buffer on the GPU."""
+    if t.dtype is _I32 and t.is_cuda and t.is_contiguous():
+        return t.data_ptr()
+    raise TypeError("contiguous int32 buffers on the GPU")
 
 
-def _pool(pool: torch.Tensor, dims: int = 5) -> tuple[int, int, int, int]:
-    """blocks, kv_heads, bs, hd of a paged cache ([layers]) [blocks][2][kv_heads][bs][hd] f16."""
-    if pool.dtype is not torch.float16 or pool.dim() != dims or pool.shape[-4] != 2 or \
+def _f32(t) -> int:
+    """The address of a contiguous float32 buffer on the GPU."""
+    if t.dtype is _F32 and t.is_cuda and t.is_contiguous():
+        return t.data_ptr()
+    raise TypeError("contiguous float32 buffers on the GPU")
+
+
+def _pool(pool: torch.Tensor, dims: int = 5):
+    """The address, blocks, kv_heads, bs and hd of a paged cache ([layers]) [blocks][2][kv_heads][bs][hd]
+    in f16."""
+    shape = pool.shape
+    if pool.dtype is not _F16 or len(shape) != dims or shape[-4] != 2 or not pool.is_cuda or \
             not pool.is_contiguous():
-        raise TypeError("a paged cache is contiguous f16 [blocks][2][kv_heads][bs][hd]")
-    blocks, _, kv_heads, bs, hd = pool.shape[-5:]
-    return blocks, kv_heads, bs, hd
+        raise TypeError("a paged cache is contiguous f16 [blocks][2][kv_heads][bs][hd] on the GPU")
+    return pool.data_ptr(), shape[-5], shape[-3], shape[-2], shape[-1]
 
 
 def pos_rows(t: int) -> int:
@@ -422,30 +427,32 @@ class Pass:
         """Block tables and the slot map of a step's rows from the requests' lengths
         (wavo_block_tables); int32 device tensors, table [n][width], row_start [n + 1], state [2],
         state_out [4] (ring head, free blocks, rows, requests refused)."""
-        n = lens.numel()
-        _int32(lens, adds, ring, state, owned, table, row_start, row_seq, slots, state_out,
-               owned_out)
-        if table.shape[0] != n or adds.numel() != n or owned.numel() != n or \
-                owned_out.numel() != n or row_start.numel() != n + 1 or state.numel() < 2 or \
-                state_out.numel() < 4 or row_seq.numel() != slots.numel():
+        n, rows = lens.numel(), slots.numel()
+        held, width = table.shape
+        if held != n or adds.numel() != n or owned.numel() != n or owned_out.numel() != n or \
+                row_start.numel() != n + 1 or state.numel() < 2 or state_out.numel() < 4 or \
+                row_seq.numel() != rows:
             raise ValueError("block_tables: sizes differ")
-        check(L.lib().wavo_block_tables(
-            self.ctx, _ptr(lens), _ptr(adds), n, bs, _ptr(ring), ring.numel(), _ptr(state),
-            _ptr(owned), _ptr(table), table.shape[1], _ptr(row_start), _ptr(row_seq), _ptr(slots),
-            slots.numel(), _ptr(state_out), _ptr(owned_out)), self.ctx)
+        status = L.lib().wavo_block_tables(
+            self.ctx, _i32(lens), _i32(adds), n, bs, _i32(ring), ring.numel(), _i32(state),
+            _i32(owned), _i32(table), width, _i32(row_start), _i32(row_seq), _i32(slots), rows,
+            _i32(state_out), _i32(owned_out))
+        if status:
+            check(status, self.ctx)
 
     def pack_slots(self, x: torch.Tensor, src_stride: tuple[int, int], slots: torch.Tensor,
                    pool: torch.Tensor) -> None:
         """`pack` for a paged cache: one row of x (f32 or f16) for each of `slots` into pool
         [blocks][2][kv_heads][bs][hd] (wavo_pack_slots)."""
-        blocks, kv_heads, bs, hd = _pool(pool)
-        _int32(slots)
+        cache, blocks, kv_heads, bs, hd = _pool(pool)
         src, stride = src_stride
         rows = slots.numel()
         if rows and src + (rows - 1) * stride + 2 * kv_heads * hd > x.numel():
             raise ValueError("pack_slots: x has fewer rows")
-        check(L.lib().wavo_pack_slots(self.ctx, _ptr(x), _dtype(x), src, stride, _ptr(slots), rows,
-                                      _ptr(pool), blocks, bs, kv_heads, hd), self.ctx)
+        status = L.lib().wavo_pack_slots(self.ctx, _ptr(x), _dtype(x), src, stride, _i32(slots), rows,
+                                         cache, blocks, bs, kv_heads, hd)
+        if status:
+            check(status, self.ctx)
 
     def attend_tree(self, q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor,
                     lens: torch.Tensor, o: torch.Tensor, max_len: int,
@@ -454,38 +461,54 @@ class Pass:
         """Attention of rows q [rows][heads * hd] over a paged cache into o (wavo_attend_tree):
         request s's rows row_start[s].. see its lens[s] positions and, with mask [rows][words], the
         drafted positions behind them whose bits are set."""
-        blocks, kv_heads, bs, hd = _pool(pool)
-        _int32(table, lens, row_start, mask)
+        cache, blocks, kv_heads, bs, hd = _pool(pool)
         rows, wide = q.shape
         n, width = table.shape
-        if q.stride(1) != 1 or o.stride(1) != 1 or o.shape != q.shape or o.dtype != q.dtype or \
-                wide % hd or lens.numel() != n or \
-                (row_start is not None and row_start.numel() != n + 1) or \
-                (mask is not None and mask.shape[0] < rows):
+        (q_row, q_el), (o_row, o_el) = q.stride(), o.stride()
+        starts = bits = None
+        words = 0
+        if row_start is not None:
+            starts = _i32(row_start)
+            if row_start.numel() != n + 1:
+                raise ValueError("attend_tree: row_start has one value more than there are requests")
+        if mask is not None:
+            bits = _i32(mask)
+            held, words = mask.shape
+            if held < rows:
+                raise ValueError("attend_tree: the mask has fewer rows")
+        if q_el != 1 or o_el != 1 or o.shape != q.shape or o.dtype is not q.dtype or wide % hd or \
+                lens.numel() != n:
             raise ValueError("attend_tree: sizes or types differ")
-        check(L.lib().wavo_attend_tree(
-            self.ctx, _ptr(q), q.stride(0), _dtype(q), _ptr(pool), blocks, bs, _ptr(table), width,
-            _ptr(row_start), _ptr(lens), n, _ptr(mask), 0 if mask is None else mask.shape[1], rows,
-            max_rows, max_len, _ptr(o), o.stride(0), wide // hd, kv_heads, hd), self.ctx)
+        status = L.lib().wavo_attend_tree(
+            self.ctx, _ptr(q), q_row, _dtype(q), cache, blocks, bs, _i32(table), width, starts,
+            _i32(lens), n, bits, words, rows, max_rows, max_len, _ptr(o), o_row, wide // hd, kv_heads,
+            hd)
+        if status:
+            check(status, self.ctx)
 
     def shape_logits(self, logits: torch.Tensor, rules: "LogitRules", picks: torch.Tensor | None,
                      logprobs: torch.Tensor | None = None, out: torch.Tensor | None = None) -> None:
         """The logits [rows][vocab] edited by the rules into out (None: not wanted; may be logits),
         their first maximum and its log-softmax (wavo_shape_logits)."""
-        rows = logits.shape[0]
-        _int32(picks)
-        rules.check(rows)
-        if logits.stride(1) != 1 or logits.shape[1] < rules.c.vocab or \
-                (out is not None and (out.stride(1) != 1 or out.dtype != logits.dtype or
-                                      out.shape[0] < rows or out.shape[1] < rules.c.vocab)) or \
+        rows, wide = logits.shape
+        ld, step = logits.stride()
+        vocab = rules.c.vocab
+        to, ld_out = None, 0
+        if out is not None:
+            ld_out, out_step = out.stride()
+            if out_step != 1 or out.dtype is not logits.dtype or out.shape[0] < rows or \
+                    out.shape[1] < vocab:
+                raise ValueError("shape_logits: sizes or types of out differ")
+            to = _ptr(out)
+        if step != 1 or wide < vocab or rules.most < rows or \
                 (picks is not None and picks.numel() < rows) or \
-                (logprobs is not None and (logprobs.numel() < rows or
-                                           logprobs.dtype != torch.float32)):
-            raise ValueError("shape_logits: sizes or types differ")
-        check(L.lib().wavo_shape_logits(
-            self.ctx, _ptr(logits), _dtype(logits), logits.stride(0), _ptr(out),
-            0 if out is None else out.stride(0), rows, ctypes.byref(rules.c), _ptr(picks),
-            _ptr(logprobs)), self.ctx)
+                (logprobs is not None and logprobs.numel() < rows):
+            raise ValueError("shape_logits: sizes differ")
+        status = L.lib().wavo_shape_logits(
+            self.ctx, _ptr(logits), _dtype(logits), ld, to, ld_out, rows, rules.ref,
+            None if picks is None else _i32(picks), None if logprobs is None else _f32(logprobs))
+        if status:
+            check(status, self.ctx)
 
     def tree_accept(self, picks: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor,
                     row_start: torch.Tensor, lens: torch.Tensor, table: torch.Tensor | None,
@@ -494,21 +517,26 @@ class Pass:
         """The drafted path that the picks confirm, and its K and V moved together in pool
         [layers][blocks][2][kv_heads][bs][hd] (None: nothing moves) (wavo_tree_accept)."""
         n, max_rows = path.shape
-        _int32(picks, tokens, mask, row_start, lens, table, path, count, next_tokens, new_lens)
-        rows = tokens.numel()
+        rows, (held, words) = tokens.numel(), mask.shape
+        cache = tables = None
         layers = layer = blocks = kv_heads = bs = hd = width = 0
-        if pool is not None:
-            layers, layer = pool.shape[0], pool.stride(0)
-            blocks, kv_heads, bs, hd = _pool(pool, 6)
+        if table is not None:
+            tables = _i32(table)
+            if table.shape[0] != n:
+                raise ValueError("tree_accept: a table a request")
             width = table.shape[1]
-        if mask.shape[0] != rows or picks.numel() < rows or row_start.numel() != n + 1 or \
-                lens.numel() != n or count.numel() != n or next_tokens.numel() != n or \
-                new_lens.numel() != n or (table is not None and table.shape[0] != n):
+        if pool is not None:
+            cache, blocks, kv_heads, bs, hd = _pool(pool, 6)
+            layers, layer = pool.shape[0], pool.stride(0)
+        if held != rows or picks.numel() < rows or row_start.numel() != n + 1 or lens.numel() != n or \
+                count.numel() != n or next_tokens.numel() != n or new_lens.numel() != n:
             raise ValueError("tree_accept: sizes differ")
-        check(L.lib().wavo_tree_accept(
-            self.ctx, _ptr(picks), _ptr(tokens), _ptr(mask), mask.shape[1], rows, _ptr(row_start),
-            n, max_rows, _ptr(lens), _ptr(table), width, _ptr(pool), layers, layer, blocks, bs,
-            kv_heads, hd, _ptr(path), _ptr(count), _ptr(next_tokens), _ptr(new_lens)), self.ctx)
+        status = L.lib().wavo_tree_accept(
+            self.ctx, _i32(picks), _i32(tokens), _i32(mask), words, rows, _i32(row_start), n, max_rows,
+            _i32(lens), tables, width, cache, layers, layer, blocks, bs, kv_heads, hd, _i32(path),
+            _i32(count), _i32(next_tokens), _i32(new_lens))
+        if status:
+            check(status, self.ctx)
 
 
 class LogitRules:
@@ -523,44 +551,39 @@ class LogitRules:
                  grammar=None, tree=None):
         self._keep = (history, penalties, bias, grammar, tree)
         c = self.c = L.LogitRulesC()
+        self.ref = ctypes.byref(c)
         sizes = [n] if n is not None else []
-        self._rows = []  # buffers with a value a row hold at least the call's rows
+        rows = []  # buffers with a value a row hold at least the call's rows
         if history is not None:
-            _int32(*history)
+            c.history, c.hist_len = map(_i32, history)
+            c.max_hist = history[0].shape[1]
             sizes += [history[0].shape[0], history[1].numel()]
-            c.history, c.hist_len, c.max_hist = *map(_ptr, history), history[0].shape[1]
         if penalties is not None:
-            if penalties.dtype != torch.float32 or penalties.shape[1] != 3:
-                raise ValueError("LogitRules: penalties are f32 [n][3]")
+            c.penalties = _f32(penalties)
+            if penalties.shape[1] != 3:
+                raise ValueError("LogitRules: penalties are [n][3]")
             sizes.append(penalties.shape[0])
-            c.penalties = _contiguous_ptr(penalties)
         if bias is not None:
             ids, vals, count = bias
-            _int32(ids, count)
-            if vals.dtype != torch.float32 or vals.shape != ids.shape:
-                raise ValueError("LogitRules: bias values are f32, as many as ids")
-            sizes += [ids.shape[0], count.numel()]
-            c.bias_ids, c.bias_vals, c.bias_len = _ptr(ids), _contiguous_ptr(vals), _ptr(count)
+            c.bias_ids, c.bias_vals, c.bias_len = _i32(ids), _f32(vals), _i32(count)
+            if vals.shape != ids.shape:
+                raise ValueError("LogitRules: as many bias values as ids")
             c.max_bias = ids.shape[1]
+            sizes += [ids.shape[0], count.numel()]
         if tree is not None:
             row_seq, row_start, tokens, path = tree
-            _int32(*tree)
-            c.row_seq, c.row_start, c.tokens, c.path = map(_ptr, tree)
+            c.row_seq, c.row_start, c.tokens, c.path = map(_i32, tree)
             c.path_words = path.shape[1]
             sizes.append(row_start.numel() - 1)
-            self._rows += [row_seq.numel(), tokens.numel(), path.shape[0]]
+            rows += [row_seq.numel(), tokens.numel(), path.shape[0]]
         if grammar is not None:
-            _int32(*grammar)
-            c.grammar, c.grammar_of = map(_ptr, grammar)
+            c.grammar, c.grammar_of = map(_i32, grammar)
             c.n_grammar, c.grammar_ld = grammar[0].shape
-            self._rows.append(grammar[1].numel())
+            rows.append(grammar[1].numel())
         if len(set(sizes)) != 1:
             raise ValueError(f"LogitRules: numbers of requests {sizes}")
         c.vocab, c.n = vocab, sizes[0]
-
-    def check(self, rows: int) -> None:
-        if self._rows and min(self._rows) < rows:
-            raise ValueError("shape_logits: a rule has fewer rows than the logits")
+        self.most = min(rows, default=1 << 31)  # rows of logits that the rules cover
 
 
 def partition_lpt(costs, parts: int) -> list[int]:
