@@ -391,3 +391,233 @@ class WhisperDecoder:
             self.logits, B, self.vocab, self.history, self.hist_len, self.suppress,
             self.n_suppress, self.begin_suppress, self.n_begin, ids["eot"], ids["no_timestamps"],
             ids["begin"], self.max_initial, self.tokens, self.logprobs))
+
+
+def tree_masks(parents) -> tuple[np.ndarray, np.ndarray]:
+    """(mask words [rows][words] as int32, depth of each row) of one request's drafted tree from its
+    rows' parents (-1 for the root, parents before children): bit j of row i is set where row j is an
+    ancestor of row i or row i itself."""
+    n = len(parents)
+    words = np.zeros((n, max(1, -(-n // 32))), np.uint32)
+    depth = np.zeros(n, np.int32)
+    for i, up in enumerate(parents):
+        if not (up == -1 and i == 0) and not 0 <= up < i:
+            raise ValueError(f"row {i} of a tree has parent {up}")
+        if i:
+            words[i] = words[up]
+            depth[i] = depth[up] + 1
+        words[i, i // 32] |= np.uint32(1 << (i % 32))
+    return words.view(np.int32), depth
+
+
+class TreeDecoder:
+    """The Whisper decoder over paged caches, verifying several drafted tokens a segment in one step
+    (no reference counterpart: the reference decodes a token a step, src/transformer.rs:254-290, which
+    is the layer stack here). A step plans the blocks and slots of its rows (`block_tables`), embeds
+    them, and per layer writes their K and V (`pack_slots`) and attends over the segment's positions and
+    each row's own path (`attend_tree`), then over the encoder's frames; the logits are shaped and
+    picked (`shape_logits`), and the path that the picks confirm stays (`tree_accept`). The tokens are
+    those that greedy decoding gives one at a time.
+
+    w, d, heads, d_ff, vocab, context, frames, batch: as WhisperDecoder's. max_rows: the rows of a
+    segment in one step at most (the longest prompt, the largest tree; up to 256). blocks: of the
+    caches of generated tokens (default: every segment's whole context). Logit rules, for all
+    segments: penalties (repetition, presence, frequency), bias {token: value}, allowed (a bool array of
+    the vocabulary, e.g. without the timestamps and Whisper's suppressed tokens)."""
+
+    def __init__(self, gpu: Gpu, ty: int, d: int, heads: int, d_ff: int, vocab: int, context: int,
+                 frames: int, batch: int, w: dict, max_rows: int, bs: int = 16, blocks: int = 0,
+                 penalties=None, bias=None, allowed=None):
+        from .gpu import LogitRules
+        self.gpu, self.d, self.heads, self.hd, self.vocab = gpu, d, heads, d // heads, vocab
+        self.context, self.frames, self.batch, self.max_rows, self.bs = context, frames, batch, max_rows, bs
+        dev = gpu.torch_device
+        up = lambda a: gpu.upload(np.asarray(a, np.float32))  # noqa: E731
+        self.embed = gpu.linear(ty, vocab, d, w["embed"], None)
+        self.positions = up(w["positions"])
+        self.norm = tuple(up(v) for v in w["norm"])
+        self.layers = []
+        for lw in w["layers"]:
+            b = lw.get("b", {})
+            lay = {k: gpu.linear(ty, n * d, d, lw[k], b.get(k)) for k, n in (
+                ("qkv", 3), ("self_out", 1), ("cross_q", 1), ("cross_kv", 2), ("cross_out", 1))}
+            lay["fc1"] = gpu.linear(ty, d_ff, d, lw["fc1"], lw.get("fc1_b"))
+            lay["fc2"] = gpu.linear(ty, d, d_ff, lw["fc2"], lw.get("fc2_b"))
+            lay.update({k: tuple(up(v) for v in lw[k]) for k in ("norm_self", "norm_cross", "norm_ffn")})
+            self.layers.append(lay)
+        i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=dev)  # noqa: E731
+        f16 = lambda *shape: torch.zeros(shape, dtype=torch.float16, device=dev)  # noqa: E731
+        rows, words, n_layers = batch * max_rows, -(-max_rows // 32), len(self.layers)
+        # The caches of generated tokens, and a segment's drafted rows past its context.
+        width = -(-(context + max_rows) // bs)
+        blocks = blocks or batch * width
+        self.pool = f16(n_layers, blocks, 2, heads, bs, self.hd)
+        self.table, self.ring = i32(batch, width), torch.arange(blocks, dtype=torch.int32, device=dev)
+        # State of the plan, before and after a step.
+        self.state, self.state_next = i32(2), i32(4)
+        self.owned, self.owned_next = i32(batch), i32(batch)
+        self.lens, self.lens_next = i32(batch), i32(batch)
+        self.state[1] = blocks
+        # The encoder's K and V: planned once, full blocks of a segment's frames.
+        cross = -(-frames // bs)
+        self.cross = f16(n_layers, batch * cross, 2, heads, bs, self.hd)
+        self.cross_table, self.cross_slots = i32(batch, cross), i32(batch * frames)
+        self.cross_lens = torch.full((batch,), frames, dtype=torch.int32, device=dev)
+        gpu.pass_().block_tables(
+            i32(batch), self.cross_lens, bs, torch.arange(batch * cross, dtype=torch.int32, device=dev),
+            torch.tensor([0, batch * cross], dtype=torch.int32, device=dev), i32(batch),
+            self.cross_table, i32(batch + 1), i32(batch * frames), self.cross_slots, i32(4), i32(batch))
+        # A step's rows.
+        self.adds, self.row_start = i32(batch), i32(batch + 1)
+        self.row_seq, self.slots, self.tokens = i32(rows), i32(rows), i32(rows)
+        self.depth, self.mask = i32(rows), i32(rows, words)
+        self.x = torch.zeros(rows, d, dtype=torch.float32, device=dev)
+        self.y, self.qkv, self.q = f16(rows, d), f16(rows, 3 * d), f16(rows, d)
+        self.att, self.h = f16(rows, d), f16(rows, d_ff)
+        self.logits = torch.zeros(rows, self.embed.width(), dtype=torch.float32, device=dev)
+        self.picks, self.logprobs = i32(rows), torch.zeros(rows, device=dev)
+        self.path, self.count, self.next = i32(batch, max_rows), i32(batch), i32(batch)
+        # The tokens in the cache, which the penalties count beside a row's path.
+        self.history = i32(batch, context + max_rows)
+        words_all = -(-vocab // 32)
+        grammar = None
+        if allowed is not None:
+            bits = np.zeros(32 * words_all, np.uint8)
+            bits[:vocab] = np.asarray(allowed, bool)
+            sets = torch.as_tensor(np.packbits(bits, bitorder="little").view(np.int32)[None]).to(dev)
+            grammar = (sets.contiguous(), i32(rows))
+        if bias:
+            ids = torch.tensor([list(bias)] * batch, dtype=torch.int32, device=dev)
+            vals = torch.tensor([list(bias.values())] * batch, dtype=torch.float32, device=dev)
+            bias = (ids, vals, torch.full((batch,), ids.shape[1], dtype=torch.int32, device=dev))
+        pen = None if penalties is None else torch.tensor(
+            [list(penalties)] * batch, dtype=torch.float32, device=dev)
+        rule = lambda lens: LogitRules(  # noqa: E731
+            vocab, n=batch, history=(self.history, lens), penalties=pen, bias=bias or None,
+            grammar=grammar, tree=(self.row_seq, self.row_start, self.tokens, self.mask))
+        self.rules, self.rules_next = rule(self.lens), rule(self.lens_next)
+
+    def record_cross(self, p: Pass, enc: torch.Tensor, chunk: int = 8) -> None:
+        """The encoder's K and V of every layer from its output [batch][frames][d] (f16 or f32);
+        chunk segments a projection."""
+        d, t = self.d, self.frames
+        kv = torch.empty(chunk * t, 2 * d, dtype=torch.float16, device=self.gpu.torch_device)
+        for layer, lay in enumerate(self.layers):
+            for b0 in range(0, self.batch, chunk):
+                rows = min(chunk, self.batch - b0) * t
+                p.gemm(enc[b0:b0 + chunk].reshape(rows, d), lay["cross_kv"], kv, rows, "bias")
+                p.pack_slots(kv, (0, 2 * d), self.cross_slots[b0 * t:b0 * t + rows], self.cross[layer])
+
+    def _record(self, p: Pass, rows: int, most: int) -> None:
+        """The step's `rows` rows through the layers, `most` of a segment at most: their picks."""
+        d, n = self.d, self.heads * self.hd
+        p.block_tables(self.lens, self.adds, self.bs, self.ring, self.state, self.owned, self.table,
+                       self.row_start, self.row_seq[:rows], self.slots[:rows], self.state_next,
+                       self.owned_next)
+        x, y, qkv, att = self.x[:rows], self.y[:rows], self.qkv[:rows], self.att[:rows]
+        p.embed_rows(self.embed, None, self.tokens, rows, 0, x)
+        at = self.lens.index_select(0, self.row_seq[:rows].clamp(min=0)) + self.depth[:rows]
+        x.add_(self.positions.index_select(0, at.clamp(max=self.context - 1)))
+        mask = self.mask[:rows]
+        longest = self.table.shape[1] * self.bs
+        for layer, lay in enumerate(self.layers):
+            p.layer_norm(x, *lay["norm_self"], y, rows, d)
+            p.gemm(y, lay["qkv"], qkv, rows, "bias")
+            p.pack_slots(qkv, (d, 3 * d), self.slots[:rows], self.pool[layer])
+            p.attend_tree(qkv[:, :n], self.pool[layer], self.table, self.lens, att, longest,
+                          row_start=self.row_start, mask=mask, max_rows=most)
+            p.gemm(att, lay["self_out"], x, rows, "residual", 1.0)
+            p.layer_norm(x, *lay["norm_cross"], y, rows, d)
+            p.gemm(y, lay["cross_q"], self.q, rows, "bias")
+            p.attend_tree(self.q[:rows], self.cross[layer], self.cross_table, self.cross_lens, att,
+                          self.frames, row_start=self.row_start, max_rows=most)
+            p.gemm(att, lay["cross_out"], x, rows, "residual", 1.0)
+            p.layer_norm(x, *lay["norm_ffn"], y, rows, d)
+            p.gemm(y, lay["fc1"], self.h, rows, "gelu")
+            p.gemm(self.h, lay["fc2"], x, rows, "residual", 1.0)
+        p.layer_norm(x, *self.norm, y, rows, d)
+        p.gemm(y, self.embed, self.logits, rows, "bias")
+        p.shape_logits(self.logits[:rows], self.rules, self.picks, self.logprobs)
+
+    def _load(self, trees) -> tuple[int, int]:
+        """The step's rows onto the device; (rows, the most of a segment)."""
+        if len(trees) != self.batch:
+            raise ValueError(f"{len(trees)} trees for {self.batch} segments")
+        made = [([], []) if t is None else t for t in trees]
+        counts = [len(tokens) for tokens, _ in made]
+        most, rows = max(counts), sum(counts)
+        if most > self.max_rows:
+            raise ValueError(f"{most} rows of a segment (at most {self.max_rows})")
+        words = np.zeros((rows, self.mask.shape[1]), np.int32)
+        depth = np.zeros(rows, np.int32)
+        at = 0
+        for (tokens, parents), c in zip(made, counts):
+            if len(parents) != c:
+                raise ValueError("as many parents as tokens")
+            if c:
+                m, dep = tree_masks(parents)
+                words[at:at + c, :m.shape[1]], depth[at:at + c] = m, dep
+                at += c
+        adds = [-1 if t is None else c for t, c in zip(trees, counts)]
+        for to, a in ((self.adds, adds), (self.tokens[:rows], [x for t, _ in made for x in t]),
+                      (self.depth[:rows], depth), (self.mask[:rows], words)):
+            to.copy_(torch.as_tensor(np.asarray(a, np.int32)))
+        return rows, most
+
+    def _keep(self, counts: torch.Tensor, rows: torch.Tensor) -> None:
+        """Takes the step's end as the next one's start; the tokens of `rows` [batch][k] (indices
+        among the step's; the first counts[b] hold) join the history."""
+        live = torch.arange(rows.shape[1], device=rows.device) < counts[:, None]
+        said = self.tokens[rows.clamp(0, self.tokens.numel() - 1).long()]
+        to = (self.lens[:, None] + torch.arange(rows.shape[1], device=rows.device)).clamp(
+            max=self.history.shape[1] - 1).long()
+        self.history.scatter_(1, to, torch.where(live, said, self.history.gather(1, to)))
+        self.state.copy_(self.state_next[:2])
+        self.owned, self.owned_next = self.owned_next, self.owned
+        self.lens, self.lens_next = self.lens_next, self.lens
+        self.rules, self.rules_next = self.rules_next, self.rules
+
+    def _refused(self) -> None:
+        short = int(self.state_next[3])
+        if short:
+            raise RuntimeError(f"{short} segments have no blocks left: give a larger `blocks`")
+
+    def start(self, p: Pass, prompts) -> list[int]:
+        """A new window: each segment's prompt tokens into its cache. Returns each segment's first
+        token. Segments that are under way give their blocks back."""
+        self.adds.fill_(-1)
+        none = self.row_seq[:0]
+        p.block_tables(self.lens, self.adds, self.bs, self.ring, self.state, self.owned, self.table,
+                       self.row_start, none, none, self.state_next, self.owned_next)
+        self.state.copy_(self.state_next[:2])
+        self.owned.copy_(self.owned_next)
+        self.lens.zero_()
+        rows, most = self._load([(list(t), list(range(-1, len(t) - 1))) for t in prompts])
+        self._record(p, rows, most)
+        self._refused()
+        counts = self.adds.clone()
+        torch.add(self.lens, counts, out=self.lens_next)
+        i = torch.arange(most, dtype=torch.int32, device=counts.device)
+        last = self.picks[(self.row_start[1:] - 1).long()].tolist()
+        self._keep(counts, self.row_start[:-1, None] + i)
+        return last
+
+    def verify(self, p: Pass, trees) -> list[list[int]]:
+        """One step. trees[b]: (tokens, parents) of segment b, tokens[0] its last decided token (parent
+        -1), the others drafted continuations, parents before children; None: the segment is done and
+        gives its blocks back. Returns the tokens each segment gains: the drafted ones that greedy decoding
+        gives too, and the one after them (none for a segment that is done; -1 where the rules leave
+        no token)."""
+        rows, most = self._load(trees)
+        if rows == 0:
+            return [[] for _ in trees]
+        self._record(p, rows, most)
+        p.tree_accept(self.picks, self.tokens[:rows], self.mask[:rows], self.row_start, self.lens,
+                      self.table, self.pool, self.path, self.count, self.next, self.lens_next)
+        self._refused()
+        out = torch.cat([self.path, self.count[:, None], self.next[:, None]], 1).tolist()
+        self._keep(self.count, self.row_start[:-1, None] + self.path)
+        gained = []
+        for t, (*path, count, after) in zip(trees, out):
+            gained.append([] if t is None or not count else [t[0][i] for i in path[1:count]] + [after])
+        return gained
