@@ -43,7 +43,9 @@ struct TreeTile {
   static constexpr int kRing = HDP == 64 ? 8 : WIDE ? 4 : 5;
   static constexpr uint32_t kOffQ = kRing * kSlot;
   static constexpr uint32_t kOffBar = kOffQ + kQBufs * kParts * kQ;
-  static constexpr uint32_t kColO = 256;                            // TMEM: S and P twice, then O
+  // TMEM: S and P twice, then O; f32's low parts sum apart (each step of a long sum drops bits of
+  // its size), and join at the end.
+  static constexpr uint32_t kColO = 256;
 };
 constexpr int TT_SOFT = 256;                                        // softmax threads
 constexpr int TT_THREADS = TT_SOFT + 96;                            // and loads, UMMAs, rows
@@ -335,14 +337,16 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
           tc_fence_after();
           const uint64_t kd = dk + uint64_t(slot * T::kSlot >> 4);
           const uint64_t qd = dq + uint64_t((k % T::kQBufs) * T::kParts * T::kQ >> 4);
+          // The low parts first: the sums are small until the high ones come, and so is what a step
+          // drops.
 #pragma unroll
-          for (int part = 0; part < T::kParts; ++part)
+          for (int part = T::kParts - 1; part >= 0; --part)
 #pragma unroll
             for (int kk = 0; kk < HDP / 16; ++kk)
               umma_f16(tmem + (g & 1) * 128,
                        qd + ((part * T::kQ + (kk >> 2) * TT_HALF + (kk & 3) * 32) >> 4),
                        kd + (((kk >> 2) * TT_HALF + (kk & 3) * 32) >> 4), id_s,
-                       part + kk > 0 ? 1u : 0u);
+                       part < T::kParts - 1 || kk > 0 ? 1u : 0u);
           umma_commit(&sh.s_full[g & 1]);
           umma_commit(&sh.empty[slot]);
           if (--left == 0) umma_commit(&sh.q_empty[k % T::kQBufs]);
@@ -360,9 +364,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
           for (int part = 0; part < T::kParts; ++part)
 #pragma unroll
             for (int kk = 0; kk < TT_KEYS / 16; ++kk)
-              umma_f16_ts(tmem + T::kColO, tmem + (j & 1) * 128 + part * 64 + kk * 8,
-                          vd + uint64_t(kk * 16 * 128 >> 4), id_o,
-                          !first_v || part + kk > 0 ? 1u : 0u);
+              umma_f16_ts(tmem + T::kColO + part * HDP, tmem + (j & 1) * 128 + part * 64 + kk * 8,
+                          vd + uint64_t(kk * 16 * 128 >> 4), id_o, !first_v || kk > 0 ? 1u : 0u);
           umma_commit(&sh.pv_done[j & 1]);
           umma_commit(&sh.empty[slot]);
         }
@@ -578,14 +581,17 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
               mbar_wait_warp(&sh.pv_done[j & 1], (j >> 1) & 1, ab, kErrTimeoutConsumer);
               tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < HDP / 2; c += 16) {
-                uint32_t o[16];
-                tmem_ld_16x2_x16<HDP / 2>(lanes + T::kColO + c, o);
-                tmem_wait_ld();
+              for (int part = 0; part < T::kParts; ++part)
+#pragma unroll 1
+                for (int c = 0; c < HDP / 2; c += 16) {
+                  const uint32_t at = lanes + T::kColO + part * HDP + c;
+                  uint32_t o[16];
+                  tmem_ld_16x2_x16<HDP / 2>(at, o);
+                  tmem_wait_ld();
 #pragma unroll
-                for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * fac);
-                tmem_st_16x2_x16<HDP / 2>(lanes + T::kColO + c, o);
-              }
+                  for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * fac);
+                  tmem_st_16x2_x16<HDP / 2>(at, o);
+                }
             }
           }
           const float base = m == -INFINITY ? 0.0f : -m;
@@ -643,6 +649,12 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
           float o[16];
 #pragma unroll
           for (int y = 0; y < 16; ++y) o[y] = __uint_as_float(u[y]);
+          if constexpr (WIDE) {
+            tmem_ld_16x2_x16<HDP / 2>(lanes + T::kColO + HDP + c, u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 16; ++y) o[y] += __uint_as_float(u[y]);
+          }
           if (odd && at >= 0) {
             const int *table = a.table + (long long)q.s * a.width;
             for (int d = 0; d < min(q.rows, 256); ++d) {

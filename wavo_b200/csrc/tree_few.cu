@@ -124,20 +124,19 @@ __device__ __forceinline__ void few_rows(const AttendTreeArgs &a, const FewItem 
     const int first = wk * KEYS;  // the warp's first position in the tile
     const int p0 = k0 + i * TF_KEYS + first;
     float sc[NT][4] = {};
+    // The low parts first: the sums are small until the high ones come, and so is what a step drops.
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int part = WIDE ? 1 : 0; part >= 0; --part)
 #pragma unroll
-      for (int n = 0; n < NT / 2; ++n) {
-        uint32_t b[4];
-        ldsm4(b, kb + tile_at(first + n * 16 + (lane >> 4) * 8 + (lane & 7),
-                              2 * ks + ((lane >> 3) & 1)));
-        mma16(sc[2 * n], qh[ks], b[0], b[1]);
-        mma16(sc[2 * n + 1], qh[ks], b[2], b[3]);
-        if constexpr (WIDE) {
-          mma16(sc[2 * n], ql[ks], b[0], b[1]);
-          mma16(sc[2 * n + 1], ql[ks], b[2], b[3]);
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int n = 0; n < NT / 2; ++n) {
+          uint32_t b[4];
+          ldsm4(b, kb + tile_at(first + n * 16 + (lane >> 4) * 8 + (lane & 7),
+                                2 * ks + ((lane >> 3) & 1)));
+          mma16(sc[2 * n], WIDE && part ? ql[ks % (WIDE ? KS : 1)] : qh[ks], b[0], b[1]);
+          mma16(sc[2 * n + 1], WIDE && part ? ql[ks % (WIDE ? KS : 1)] : qh[ks], b[2], b[3]);
         }
-      }
     bool odd = false;  // a V row that some rows do not see holds an infinity or NaN
     if (!(bits >> 31)) {
       // Positions past the end, outside the pool, or drafted off a row's path.
