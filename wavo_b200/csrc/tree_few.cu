@@ -1,12 +1,20 @@
-// attend_tree for few rows: up to 64 rows that read one K and V head (its drafted rows and the heads
-// that share it). The steps from a tile's arrival to its sums are then short and the tiles of a request
-// few, so what counts is how many of them are under way at once: registers hold everything between
-// the products (mma.sync), no tensor memory and no hand-over between warps, and three or four CTAs share an SM.
+// attend_tree for few rows: an item is one K and V head of one request with the rows that read it (its
+// drafted rows and the heads that share it), 64 at most in a CTA. The steps from a tile's arrival to its
+// sums are then short and the tiles of a request few, so what counts is how many of them are under way
+// at once: mma.sync with everything in registers between the products, no tensor memory, no hand-over
+// between warps, and 2 to 5 CTAs an SM. The form with tcgen05 (tree.cu) takes over where the products
+// would bound it; the figures of both are beside the rule there.
 //
 // One pass over K and V with the softmax's running maximum and sum: a CTA takes an item's rows over a
 // range of positions. A producer warp loads 64 positions at a time, page by page, through TMA boxes
 // that follow the block table; four warps multiply. 16 rows a warp: where the item has fewer than 64,
 // the warps share a tile's positions instead, and meet in shared memory at the end.
+//
+// Bound by the loads: 32 x 20 items of 16 rows over 1500 positions (246 MB, f16) take 46 us, 5.3 TB/s; the same
+// loads without the products took 54 us in CTAs of their own. One f32 row an item over 448 positions at
+// most (34 MB) 18 us, of which launch and the first page's way (row starts, table, K) are most. 64 f32 rows an
+// item over 448 positions (two products each way) 52 us, bound by the latency of 12 warps an SM. Two stages and
+// five CTAs instead of three and four: 62 -> 50 us at the first; Q in shared memory, not registers: 50 -> 46.
 #include <algorithm>
 #include <type_traits>
 
@@ -57,9 +65,10 @@ __device__ __forceinline__ void warps_sync() {
 template <int HDP, int MAXR, bool WIDE>
 struct FewTile {
   static constexpr uint32_t kStage = 2 * (HDP / 64) * TF_HALF;
-  static constexpr int kStages = HDP == 64 && MAXR == 64 ? 3 : 2;
-  static constexpr int kCtas = HDP == 128 ? 2 : MAXR == 64 || WIDE ? 3 : 5;  // of an SM
-  static constexpr size_t kSmem = kStages * kStage + 1024;
+  static constexpr int kStages = 2;
+  static constexpr int kCtas = HDP == 128 ? 2 : MAXR == 16 ? 5 : WIDE ? 3 : 4;  // of an SM
+  static constexpr size_t kSmem =
+      kStages * kStage + (WIDE ? 2 : 1) * (HDP / 64) * MAXR * 128 + 1024;
 };
 
 template <int ST>
@@ -96,22 +105,42 @@ __device__ __forceinline__ void few_rows(const AttendTreeArgs &a, const FewItem 
     row[u] = r < f.rows && f.lo + i < a.rows ? f.lo + i : -1;
     seen[u] = a.mask && row[u] >= 0 ? a.mask[(long long)row[u] * a.words] : 0u;
   }
-  uint32_t qh[KS][4], ql[WIDE ? KS : 1][4];
+  // Q into shared memory behind the tiles, rows of 128 bytes in the tiles' swizzle, f32's low parts
+  // after the high ones: registers for it would cost a CTA an SM.
+  const uint32_t qs = smem_u32(tiles + ST * STAGE);
+  constexpr uint32_t Q_HALF = MT * 128, Q_PART = (HDP / 64) * Q_HALF;
+  {
+    const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (a.q_stride * sizeof(E))) & 15u) == 0;
+    for (int e = tid; e < MT * (HDP / 8); e += TF_WARPS * 32) {
+      const int r = e / (HDP / 8), c = e % (HDP / 8), i = (f.r0 + r) / group;
+      E v[8];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
+      for (int x = 0; x < 8; ++x) v[x] = E(0.0f);
+      if (f.r0 + r < f.rows && f.lo + i < a.rows && c * 8 < a.hd) {
+        const int head = f.kvh * group + (f.r0 + r) - i * group;
+        const E *from = static_cast<const E *>(a.q) + (f.lo + i) * a.q_stride + head * a.hd + c * 8;
+        if (vec) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int u = x & 1, c = 16 * ks + c2 + 8 * (x >> 1);
-      const int head = f.kvh * group + (f.r0 + wr * 16 + g + 8 * u) % group;
-      E v[2] = {E(0.0f), E(0.0f)};
-      if (row[u] >= 0 && c < a.hd) {
-        const E *p = static_cast<const E *>(a.q) + row[u] * a.q_stride + head * a.hd + c;
-        v[0] = p[0];
-        v[1] = p[1];
+          for (int x = 0; x < int(sizeof(E)) / 2; ++x)
+            reinterpret_cast<uint4 *>(v)[x] = reinterpret_cast<const uint4 *>(from)[x];
+        } else {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[x] = from[x];
+        }
       }
-      if constexpr (WIDE) split2(v[0], v[1], qh[ks][x], ql[ks][x]);
-      else qh[ks][x] = uint32_t(__half_as_ushort(v[0])) | uint32_t(__half_as_ushort(v[1])) << 16;
+      uint8_t *to = tiles + ST * STAGE + (c >> 3) * Q_HALF + sw128_offset(r, c & 7);
+      if constexpr (WIDE) {
+        uint32_t hi[4], low[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) split2(v[2 * x], v[2 * x + 1], hi[x], low[x]);
+        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(to + Q_PART) = make_uint4(low[0], low[1], low[2], low[3]);
+      } else {
+        *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(v);
+      }
     }
+    warps_sync();
+  }
   float acc[2 * KS][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   const float scale = a.scale * 1.4426950408889634f;  // exponentials of base 2
   bool ok = true;
@@ -128,15 +157,19 @@ __device__ __forceinline__ void few_rows(const AttendTreeArgs &a, const FewItem 
 #pragma unroll
     for (int part = WIDE ? 1 : 0; part >= 0; --part)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t qf[4];
+        ldsm4(qf, qs + part * Q_PART + (ks >> 2) * Q_HALF +
+                      sw128_offset(wr * 16 + (lane & 15), (2 * ks + (lane >> 4)) & 7));
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) {
           uint32_t b[4];
           ldsm4(b, kb + tile_at(first + n * 16 + (lane >> 4) * 8 + (lane & 7),
                                 2 * ks + ((lane >> 3) & 1)));
-          mma16(sc[2 * n], WIDE && part ? ql[ks % (WIDE ? KS : 1)] : qh[ks], b[0], b[1]);
-          mma16(sc[2 * n + 1], WIDE && part ? ql[ks % (WIDE ? KS : 1)] : qh[ks], b[2], b[3]);
+          mma16(sc[2 * n], qf, b[0], b[1]);
+          mma16(sc[2 * n + 1], qf, b[2], b[3]);
         }
+      }
     bool odd = false;  // a V row that some rows do not see holds an infinity or NaN
     if (!(bits >> 31)) {
       // Positions past the end, outside the pool, or drafted off a row's path.
