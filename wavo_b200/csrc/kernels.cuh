@@ -187,7 +187,7 @@ cudaError_t launch_gemv(const float *a, long long lda, int wtype, const void *w,
 
 struct BlockTablesArgs {
   const int *lens, *adds;  // [n]: positions held; rows of this step, negative: the request is done
-  int n, bs;
+  int n, bs, shift;        // bs = 1 << shift
   int *ring;               // ids of free blocks, `cap` of them, used as a ring
   int cap;
   const int *state;        // {ring head, free blocks}

@@ -1585,9 +1585,24 @@ wavo_status wavo_block_tables(wavo_ctx *ctx, const int32_t *lens, const int32_t 
   if (state == state_out || owned == owned_out)
     return fail(ctx, WAVO_EINVAL, "block_tables: state_out and owned_out need buffers of their own");
   cudaSetDevice(ctx->device);
-  const wv::BlockTablesArgs a = {lens,  adds,      int(n),  int(bs), ring,       int(ring_cap),
-                                 state, state_out, owned,   owned_out, table,    int(width),
-                                 row_start, row_seq, slots, int(rows_cap)};
+  wv::BlockTablesArgs a = {};
+  a.lens = lens;
+  a.adds = adds;
+  a.n = int(n);
+  a.bs = int(bs);
+  while ((1u << a.shift) < bs) ++a.shift;
+  a.ring = ring;
+  a.cap = int(ring_cap);
+  a.state = state;
+  a.state_out = state_out;
+  a.owned = owned;
+  a.owned_out = owned_out;
+  a.table = table;
+  a.width = int(width);
+  a.row_start = row_start;
+  a.row_seq = row_seq;
+  a.slots = slots;
+  a.rows_cap = int(rows_cap);
   CK(wv::launch_block_tables(a, ctx->sms, ctx->stream), "block_tables launch");
   return WAVO_OK;
 }
