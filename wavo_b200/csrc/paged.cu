@@ -21,7 +21,9 @@ namespace {
 //
 // One launch and no hand-over between CTAs: a CTA takes `per` consecutive requests, sums what
 // the others before it need (and what all do) from the 12 bytes of each, and scans its own. A few
-// microseconds of latency, not bytes, bound it: at 2048 requests every CTA reads 24 KB out of L2.
+// microseconds of latency, not bytes, bound it: at 2048 requests every CTA reads 24 KB out of L2. 32 requests
+// of 16 rows take 6.7 us on the device from cold caches, 2048 requests of up to 96 rows 16 us; a call from
+// Python costs the host 8 to 10 us.
 constexpr int BT_THREADS = 256;
 
 struct BtNeed {
@@ -208,8 +210,9 @@ __global__ void __launch_bounds__(BT_THREADS) block_tables_kernel(const BlockTab
 
 // ---- K and V rows into the cache ----------------------------------------------------------
 
-// Eight elements a thread and row (one 16-byte store); a thread keeps its place in the row and walks
-// down the rows, so that the head and the element are divided out once.
+// Eight elements a thread and row (one 16-byte store); a thread keeps its place in the row, so that
+// the head and the element are divided out once. Bound by the memory: 48000 f32 rows of 2560 (737 MB)
+// take 126 us, 5.9 TB/s, 0.91 of the measured copy.
 template <typename T, bool VEC>
 __device__ __forceinline__ uint4 load8(const T *p) {
   uint4 o;
@@ -266,8 +269,8 @@ __global__ void __launch_bounds__(256)
 // consecutive positions. path[k] >= k and rises, so no destination is the source of a later move,
 // and a thread that keeps its place in the head and walks k upwards needs no barrier.
 // A chain of latencies (row starts, tokens, the walk, table entries, one load and store) bounds it: 128
-// requests of up to 64 nodes over 4 layers (2.6 MB) took 13.6 us with a move's store before the next
-// move's load.
+// requests of up to 64 nodes over 4 layers take 9 to 12 us on the device from cold caches, and took 16 to 20
+// with each move's store before the next move's load.
 constexpr int TA_THREADS = 256;
 constexpr int TA_MAX = 256;  // nodes of a tree
 constexpr int TA_BATCH = 8;

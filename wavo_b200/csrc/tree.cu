@@ -17,6 +17,13 @@
 // many CTAs as are resident: ragged lengths, few long requests and many short ones fill the GPU alike,
 // and the loads run ahead across the items of a run. A run that ends inside an item leaves its part in
 // global memory, and a second kernel joins an item's parts in the order of the runs.
+//
+// Two requests of up to 131072 positions, 8 K and V heads of 128 and up to 96 rows each (685 MB, 53 GFLOP):
+// 143 us and 9 for the join, 4.8 TB/s; the loads alone, in the same runs, take 137 to 157. A tile costs the
+// softmax warps about 2300 cycles (the exponentials 770 of them) and its 64 KB an SM's share of the memory
+// 2800; at the clocks that the power limit leaves the two are close. Positions as the UMMA's M and the rows as
+// its N (P through shared memory, a vote of all warps a tile) took 215 us, the join by the last CTA alone 57
+// more.
 #include <algorithm>
 #include <type_traits>
 
