@@ -534,6 +534,38 @@ def test_on_another_stream_and_in_a_graph(gpu):
     assert torch.equal(o, first)
 
 
+@pytest.mark.parametrize("heads,t", [(4, 3), (32, 24)])   # one kernel of the attention each
+def test_scratch_before_a_capture(heads, t):
+    from wavo_b200 import WavoError
+    from wavo_b200.gpu import Gpu
+    rng = np.random.default_rng(21)
+    n, hd, kvh, bs, most = 2, 64, 4, 16, 6000
+    lens, rows = [5000, 700], 2 * t
+    mask, _ = R.random_trees(rng, [t] * n, 1)
+    table, blocks = R.paged(rng, [a + t for a in lens], bs)
+    pool = torch.randn(blocks, 2, kvh, bs, hd, device="cuda").half()
+    q = torch.randn(rows, heads * hd, device="cuda").half()
+    want, o = torch.empty_like(q), torch.empty_like(q)
+    tb, ln, starts, m = i32(table), i32(lens), i32([0, t, rows]), words(mask)
+    g = Gpu(0)
+    go = lambda p, to: p.attend_tree(q, pool, tb, ln, to, most, row_start=starts, mask=m,  # noqa: E731
+                                     max_rows=t)
+    with pytest.raises(WavoError, match="wavo_reserve"):
+        g.capture(lambda p: go(p, o))
+    need = g.attend_tree_scratch(n, rows, t, most, heads, kvh, hd)
+    assert need > 0
+    g.reserve(need)
+    graph = g.capture(lambda p: go(p, o))
+    go(g.pass_(), want)
+    graph.launch()
+    g.sync()
+    assert torch.equal(o, want)
+    ref, terms = R.attend(q.cpu().numpy(), pool.cpu().numpy(), table, [0, t, rows], lens, mask, heads)
+    hold(o.double().cpu().numpy(), ref, terms, "f16")
+    del graph
+    g.close()
+
+
 def refused(gpu, call, what):
     from wavo_b200 import WavoError, _lib as L
     with pytest.raises(WavoError) as e:

@@ -230,6 +230,12 @@ class Gpu:
     def reserve(self, nbytes: int) -> None:
         check(L.lib().wavo_reserve(self.ctx, nbytes), self.ctx)
 
+    def attend_tree_scratch(self, n: int, rows: int, max_rows: int, max_len: int, heads: int,
+                            kv_heads: int, hd: int) -> int:
+        """Bytes of scratch that such an `attend_tree` needs (`reserve` them before a capture)."""
+        return int(L.lib().wavo_attend_tree_scratch(self.ctx, n, rows, max_rows, max_len, heads,
+                                                    kv_heads, hd))
+
     def set_q8_gemm(self, mode: int) -> int:
         """How Q8_0 layers' GEMMs read W (L.Q8_AUTO, L.Q8_DEQUANT, L.Q8_PROLOGUE); returns the
         previous mode."""
