@@ -382,11 +382,12 @@ wavo_status wavo_pack_slots(wavo_ctx *ctx, const void *x, int x_dtype, uint32_t 
  * lens[s] positions alone (a single token whose K and V are packed already, or the queries of a
  * cross attention over the encoder frames). row_start NULL: request s has the one row s. Head h reads
  * K and V head h / (heads / kv_heads). max_rows is at least the rows of every request (at most
- * 32 * mask_words with a mask), max_len at least every number of positions. Scores are scaled by
- * 1 / sqrt(hd). A row that sees nothing gets zeros; what a row does not see has no effect on it,
- * whatever it holds. WAVO_F16: f16 products, f32 sums, probabilities rounded to f16 before they
- * meet V. WAVO_F32: q and the probabilities enter as two f16 parts each, f32 accuracy (q below
- * f16's largest value). Table entries outside the pool are positions that no row sees.
+ * 32 * mask_words with a mask), max_len at least every number of positions, cached and drafted
+ * (what lies beyond is not seen). Scores are scaled by 1 / sqrt(hd). A row that sees nothing gets
+ * zeros; what a row does not see has no effect on it, whatever it holds. WAVO_F16: f16 products,
+ * f32 sums, probabilities rounded to f16 before they meet V. WAVO_F32: q and the probabilities enter
+ * as two f16 parts each, f32 accuracy (q below f16's largest value). Table entries outside the pool
+ * are positions that no row sees.
  * wavo_attend_tree_scratch is the scratch that a call needs (see wavo_reserve). */
 wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, int dtype,
                              const void *pool, uint32_t blocks, uint32_t bs, const int32_t *table,

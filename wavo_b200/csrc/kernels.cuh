@@ -226,7 +226,8 @@ struct AttendTreeArgs {
   const int *lens;       // [n]
   const uint32_t *mask;  // [rows][words]; nullptr: no drafted positions
   int words;
-  int rows, max_rows, max_len;
+  int rows, max_rows;
+  int max_len;           // positions that count at most, no more than the tables reach
   int heads, kv_heads, hd;
   float scale;           // 1 / sqrt(hd)
   int n;                 // requests
@@ -235,7 +236,7 @@ struct AttendTreeArgs {
   TreeJoin *joins;       // many rows: one a run
   int *err;              // device error word
 };
-// Few rows (tree_few.cu): every request, K and V head and 64 rows has `splits` CTAs, over `chunk`
+// Few rows (tree_few.cu): every request, K and V head and 32 rows has `splits` CTAs, over `chunk`
 // positions each. map: as below, boxes of min(bs, 64) positions.
 struct AttendFewPlan {
   int splits, chunk;
@@ -247,7 +248,7 @@ cudaError_t launch_attend_few(const CUtensorMap &map, const AttendTreeArgs &a, i
                               cudaStream_t s);
 // Many rows (tree.cu).
 // Whether a call goes to the few-rows kernel.
-bool attend_tree_few(int max_rows, int max_len, int heads, int kv_heads, int hd);
+bool attend_tree_few(int max_rows, int max_len, int heads, int kv_heads);
 size_t attend_tree_part_bytes(int hd, int sms);
 // map: the pool as a 4D f16 tensor {hd, bs, 2 kv_heads, blocks}, boxes {64, min(bs, 128), 1, 1},
 // 128-byte swizzle, zeros outside.

@@ -96,7 +96,7 @@ __device__ __forceinline__ TreeRequest tree_request(const AttendTreeArgs &a, int
   r.rows = min(a.row_start ? a.row_start[s + 1] - r.lo : 1, a.max_rows);
   if (r.lo < 0 || r.rows < 0) r.rows = 0;
   r.len = max(a.lens[s], 0);
-  r.keys = int(min((long long)r.len + (a.mask ? r.rows : 0), (long long)a.width * a.bs));
+  r.keys = int(min((long long)r.len + (a.mask ? r.rows : 0), (long long)a.max_len));
   r.row_tiles = (r.rows * (a.heads / a.kv_heads) + TT_ROWS - 1) / TT_ROWS;
   r.tiles = max((r.keys + TT_KEYS - 1) / TT_KEYS, 1);
   return r;
@@ -789,15 +789,13 @@ cudaError_t launch_tile(const CUtensorMap &map, const AttendTreeArgs &a, int sms
 
 }  // namespace
 
-// Measured on both sides (us, f16 / f32, few : many; 2 x 16384 positions unless said otherwise):
-// heads of 128: 24 rows 33 : 34 / 45 : 42, 48 rows 57 : 40 / 84 : 53, 96 rows 81 : 53 / 119 : 74;
-// heads of 64: 24 rows 37 : 50 / 49 : 59, 48 rows 56 : 58 / 83 : 65, 96 rows 84 : 56 / 143 : 83, but over 16 x 1024
-// positions 96 rows 57 : 66 / 70 : 81, and 128 rows of 32 x 512 103 : 135 (f32).
-bool attend_tree_few(int max_rows, int max_len, int heads, int kv_heads, int hd) {
+// Measured on both sides, us few : many, f16 and f32. Long: 2 x 16384 positions, heads of 128: 32 rows 38 : 38, 46 : 49;
+// 48 rows 47 : 40, 62 : 53; 96 rows 70 : 53, 90 : 73; heads of 64: 32 rows 43 : 53, 54 : 57; 48 rows 66 : 57, 99 : 65. 32 x
+// 1500, heads of 64: 48 rows 95 : 87, 116 : 120; 96 rows 135 : 102, 176 : 155. Short: 32 x 512, heads of 128: 64 rows
+// 42 : 50, 48 : 74; 128 rows 66 : 74, 93 : 96; 192 rows 117 : 76, 118 : 124; heads of 64: 96 rows 62 : 63, 72 : 149.
+bool attend_tree_few(int max_rows, int max_len, int heads, int kv_heads) {
   const long long rows = (long long)max_rows * (heads / kv_heads);
-  if (rows <= 32) return true;
-  if (hd > 64 || rows > 128) return false;
-  return max_len < (rows > 64 ? 1280 : 2048);
+  return rows <= 32 || (rows <= 128 && max_len < 1280);
 }
 
 size_t attend_tree_part_bytes(int hd, int sms) {

@@ -1,5 +1,5 @@
 // attend_tree for few rows: an item is one K and V head of one request with the rows that read it (its
-// drafted rows and the heads that share it), 64 at most in a CTA. The steps from a tile's arrival to its
+// drafted rows and the heads that share it), 32 at most in a CTA. The steps from a tile's arrival to its
 // sums are then short and the tiles of a request few, so what counts is how many of them are under way
 // at once: mma.sync with everything in registers between the products, no tensor memory, no hand-over
 // between warps, and 2 to 5 CTAs an SM. The form with tcgen05 (tree.cu) takes over where the products
@@ -7,14 +7,16 @@
 //
 // One pass over K and V with the softmax's running maximum and sum: a CTA takes an item's rows over a
 // range of positions. A producer warp loads 64 positions at a time, page by page, through TMA boxes
-// that follow the block table; four warps multiply. 16 rows a warp: where the item has fewer than 64,
-// the warps share a tile's positions instead, and meet in shared memory at the end.
+// that follow the block table; four warps multiply, 16 rows each: they share a tile's positions, and meet in
+// shared memory at the end.
 //
 // Bound by the loads: 32 x 20 items of 16 rows over 1500 positions (246 MB, f16) take 46 us, 5.3 TB/s; the same
 // loads without the products took 54 us in CTAs of their own. One f32 row an item over 448 positions at
-// most (34 MB) 18 us, of which launch and the first page's way (row starts, table, K) are most. 64 f32 rows an
-// item over 448 positions (two products each way) 52 us, bound by the latency of 12 warps an SM. Two stages and
-// five CTAs instead of three and four: 62 -> 50 us at the first; Q in shared memory, not registers: 50 -> 46.
+// most (34 MB) 18 us, of which launch and the first page's way (row starts, table, K) are most. Up to 64 f32 rows an
+// item over 448 positions (two products each way) 45 us, bound by the latency of 16 warps an SM; 64 rows a CTA, a
+// page read once, took 52 (three CTAs an SM), 16 rows a CTA 45, but 33 for 25 us where 32 rows have 1500
+// positions. Two stages and five CTAs instead of three and four: 62 -> 50 us at the first; Q in shared memory,
+// not registers: 50 -> 46.
 #include <algorithm>
 #include <type_traits>
 
@@ -26,7 +28,7 @@ namespace {
 constexpr int TF_KEYS = 64;                  // positions a tile
 constexpr int TF_WARPS = 4;                  // multiplying warps
 constexpr int TF_THREADS = TF_WARPS * 32 + 32;
-constexpr int TF_ROWS = 64;                  // rows of a CTA at most
+constexpr int TF_ROWS = 32;                  // rows of a CTA at most
 constexpr uint32_t TF_HALF = TF_KEYS * 128;  // bytes of 64 positions x 64 elements
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
@@ -61,12 +63,12 @@ __device__ __forceinline__ void warps_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(TF_WARPS * 32) : "memory");
 }
 
-// MAXR: rows that a CTA can have, 16 or 64. WIDE: f32 rows, as two f16 parts each.
+// MAXR: rows that a CTA can have, 16 or 32. WIDE: f32 rows, as two f16 parts each.
 template <int HDP, int MAXR, bool WIDE>
 struct FewTile {
   static constexpr uint32_t kStage = 2 * (HDP / 64) * TF_HALF;
   static constexpr int kStages = 2;
-  static constexpr int kCtas = HDP == 128 ? 2 : MAXR == 16 ? 5 : WIDE ? 3 : 4;  // of an SM
+  static constexpr int kCtas = HDP == 128 ? 2 : MAXR == 16 ? 5 : 4;  // of an SM
   static constexpr size_t kSmem =
       kStages * kStage + (WIDE ? 2 : 1) * (HDP / 64) * MAXR * 128 + 1024;
 };
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(TF_THREADS, FewTile<HDP, MAXR, WIDE>::kCtas)
   f.rows = t * (a.heads / a.kv_heads);  // token by token, the heads of each together
   if (f.r0 >= f.rows || f.lo < 0) return;
   f.len = max(a.lens[f.s], 0);
-  const int keys = int(min((long long)f.len + (a.mask ? t : 0), (long long)a.width * a.bs));
+  const int keys = int(min((long long)f.len + (a.mask ? t : 0), (long long)a.max_len));
   f.k0 = f.split * a.chunk;
   f.k1 = min(keys, f.k0 + a.chunk);
   f.n_tiles = f.k1 > f.k0 ? (f.k1 - f.k0 + TF_KEYS - 1) / TF_KEYS : 0;
@@ -444,8 +446,7 @@ __global__ void __launch_bounds__(TF_THREADS, FewTile<HDP, MAXR, WIDE>::kCtas)
   }
   const int here = f.rows - f.r0;
   if (MAXR == 16 || here <= 16) few_rows<HDP, ST, 1, WIDE>(a, f, tiles, sh, ab);
-  else if (here <= 32) few_rows<HDP, ST, 2, WIDE>(a, f, tiles, sh, ab);
-  else few_rows<HDP, ST, 4, WIDE>(a, f, tiles, sh, ab);
+  else few_rows<HDP, ST, 2, WIDE>(a, f, tiles, sh, ab);
 }
 
 // The ranges of a row joined: a CTA a (drafted row, request), four elements a thread.

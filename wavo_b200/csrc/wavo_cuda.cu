@@ -1691,7 +1691,7 @@ wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, in
   a.err = ctx->dev_err;
   const int f16 = dtype == WAVO_F16;
   const bool few =
-      wv::attend_tree_few(int(max_rows), a.max_len, int(heads), int(kv_heads), int(hd));
+      wv::attend_tree_few(int(max_rows), a.max_len, int(heads), int(kv_heads));
   size_t bytes;
   if (few) {
     const wv::AttendFewPlan plan = wv::attend_few_plan(int(n), int(max_rows), a.max_len, int(heads),
