@@ -386,7 +386,8 @@ wavo_status wavo_pack_slots(wavo_ctx *ctx, const void *x, int x_dtype, uint32_t 
  * (what lies beyond is not seen). Scores are scaled by 1 / sqrt(hd). A row that sees nothing gets
  * zeros; what a row does not see has no effect on it, whatever it holds. WAVO_F16: f16 products,
  * f32 sums, probabilities rounded to f16 before they meet V. WAVO_F32: q and the probabilities enter
- * as two f16 parts each, f32 accuracy (q below f16's largest value). Table entries outside the pool
+ * as two f16 parts each, for f32 accuracy (q below f16's largest value; measured against 64 bits:
+ * relative 2-norms of 2e-7 to 3e-6, growing with the positions). Table entries outside the pool
  * are positions that no row sees.
  * wavo_attend_tree_scratch is the scratch that a call needs (see wavo_reserve). */
 wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, int dtype,

@@ -232,6 +232,84 @@ def test_attend_tree_branches_do_not_touch_one_another(gpu, dtype, kind):
         assert torch.isnan(after[~blind]).all()
 
 
+# The kernel for many rows (more than 128 of a K and V head, or more than 32 over a long cache).
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128, 40])
+def test_attend_tree_many_rows_any_mask(gpu, dtype, hd):
+    rng = np.random.default_rng(30)
+    counts, lens = [40, 7, 0, 64, 12, 1], [0, 0, 5, 90, 0, 700]
+    mask = rng.integers(0, 2 ** 32, (sum(counts), 2), dtype=np.uint32)
+    mask[rng.random(len(mask)) < 0.3] = 0
+    mask[-13:-1] = 0
+    got, want, terms = attend_case(gpu, 2, dtype, counts, lens, 16, 2, hd, 16, mask)
+    hold(got, want, terms, dtype)
+    assert (got[-13:-1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kvh,hd,n,t,bs", [
+    (8, 1, 128, 5000, 12, 32), (6, 1, 64, 9001, 9, 8), (40, 4, 80, 1300, 20, 256), (5, 1, 64, 20000, 8, 64)])
+def test_attend_tree_many_rows_long(gpu, dtype, heads, kvh, hd, n, t, bs):
+    rng = np.random.default_rng(n)
+    counts, lens = [t, 3, t // 2], [n, n // 3, 130]
+    mask, _ = R.random_trees(rng, counts, 1)
+    hold(*attend_case(gpu, n, dtype, counts, lens, heads, kvh, hd, bs, mask, spoil=n < 2000), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("strides", [(8, 8), (1, 3)])
+def test_attend_tree_many_rows_strides(gpu, dtype, strides):
+    rng = np.random.default_rng(31)
+    counts, lens = [20, 4], [77, 300]
+    mask, _ = R.random_trees(rng, counts, 1)
+    hold(*attend_case(gpu, 6, dtype, counts, lens, 16, 2, 64, 16, mask, strides=strides), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("kind", ["nan", "inf", "large"])
+def test_attend_tree_many_rows_branches_do_not_touch_one_another(gpu, dtype, kind):
+    rng = np.random.default_rng(32)
+    t, n, hd, bs, heads = 20, 150, 64, 16, 16
+    mask, _ = R.random_trees(rng, [t], 1)
+    table, blocks = R.paged(rng, [n + t], bs)
+    pool = torch.as_tensor(rng.standard_normal((blocks, 2, 2, bs, hd)).astype(np.float16)).cuda()
+    q = torch.as_tensor(rng.standard_normal((t, heads * hd))).to(TYPES[dtype]).cuda()
+    node = 4
+
+    def go():
+        o = torch.empty_like(q)
+        gpu.pass_().attend_tree(q, pool, i32(table), i32([n]), o, n + t, row_start=i32([0, t]),
+                                mask=words(mask), max_rows=t)
+        gpu.sync()
+        return o
+    before = go()
+    v = {"nan": float("nan"), "inf": float("inf"), "large": 65504.0}[kind]
+    pool[table[0, (n + node) // bs], :, :, (n + node) % bs] = v
+    after = go()
+    blind = torch.as_tensor([not R.sees(m, node) for m in mask]).cuda()
+    assert blind.sum() > 4 and (~blind).sum() > 2
+    assert torch.equal(before[blind], after[blind])
+    if kind == "nan":
+        assert torch.isnan(after[~blind]).all()
+
+
+def test_attend_tree_positions_past_max_len_are_not_seen(gpu):
+    rng = np.random.default_rng(33)
+    for heads, t in ((4, 3), (16, 20)):
+        n, hd, bs, most = 300, 64, 16, 200
+        table, blocks = R.paged(rng, [n], bs)
+        pool = rng.standard_normal((blocks, 2, 2, bs, hd)).astype(np.float16)
+        q = rng.standard_normal((t, heads * hd)).astype(np.float32)
+        qd = torch.as_tensor(q).cuda()
+        o = torch.empty_like(qd)
+        gpu.pass_().attend_tree(qd, torch.as_tensor(pool).cuda(), i32(table), i32([n]), o, most,
+                                row_start=i32([0, t]), max_rows=t)
+        gpu.sync()
+        want, terms = R.attend(q, pool, table, [0, t], [most], None, heads)
+        hold(o.double().cpu().numpy(), want, terms, "f32")
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("heads,kvh,hd,n", [(8, 2, 128, 5000), (4, 4, 64, 9001), (1, 1, 64, 30000)])
 def test_attend_tree_long(gpu, dtype, heads, kvh, hd, n):

@@ -160,6 +160,22 @@ def test_decoder_runs_out_of_blocks(gpu_or_new):
     assert len(dec.verify(p, [([first[0]], [-1]), None])[0]) == 1
 
 
+def test_tokens_and_trees_are_checked_before_the_device(gpu_or_new):
+    from wavo_b200 import GGML_F16
+    from wavo_b200.blocks import TreeDecoder
+    p = gpu_or_new.pass_()
+    dec = TreeDecoder(gpu_or_new, GGML_F16, D, HEADS, D_FF, VOCAB, CONTEXT, FRAMES, 2,
+                      encode(weights(np.random.default_rng(3))), 8)
+    dec.record_cross(p, torch.zeros(2, FRAMES, D, device="cuda"))
+    one = ([1], [-1])
+    for bad in ([([VOCAB], [-1]), one], [([-1], [-1]), one], [([1, 2], [-1]), one], [one],
+                [([1] * 9, list(range(-1, 8))), one], [([1, 2], [-1, 1]), one]):
+        with pytest.raises(ValueError):
+            dec.verify(p, bad)
+    assert len(dec.start(p, [[1], [2, 3]])) == 2
+    gpu_or_new.sync()
+
+
 def test_trees_are_checked(gpu_or_new):
     from wavo_b200.blocks import tree_masks
     m, depth = tree_masks([-1, 0, 0, 2])

@@ -554,6 +554,8 @@ class TreeDecoder:
         for (tokens, parents), c in zip(made, counts):
             if len(parents) != c:
                 raise ValueError("as many parents as tokens")
+            if not all(0 <= t < self.vocab for t in tokens):
+                raise ValueError(f"a token outside the {self.vocab} of the vocabulary")
             if c:
                 m, dep = tree_masks(parents)
                 words[at:at + c, :m.shape[1]], depth[at:at + c] = m, dep

@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(TA_THREADS) tree_accept_kernel(const TreeAccep
   const int *table = a.table + (long long)s * a.width;
   const auto place = [&](int pos) -> long long {
     const int blk = pos / a.bs;
-    if (blk >= a.width) return -1;
+    if (pos < 0 || blk >= a.width) return -1;
     const int b = table[blk];
     return b < 0 || b >= a.blocks ? -1 : b * block + (long long)(pos - blk * a.bs) * a.hd;
   };

@@ -13,8 +13,8 @@
 // Bound by the loads: 32 x 20 items of 16 rows over 1500 positions (246 MB, f16) take 46 us, 5.3 TB/s; the same
 // loads without the products took 54 us in CTAs of their own. One f32 row an item over 448 positions at
 // most (34 MB) 18 us, of which launch and the first page's way (row starts, table, K) are most. Up to 64 f32 rows an
-// item over 448 positions (two products each way) 45 us, bound by the latency of 16 warps an SM; 64 rows a CTA, a
-// page read once, took 52 (three CTAs an SM), 16 rows a CTA 45, but 33 for 25 us where 32 rows have 1500
+// item over 448 positions (two products each way) 47 us, bound by the latency of 16 warps an SM; 64 rows a CTA, a
+// page read once, took 7 more (three CTAs an SM), 16 rows a CTA as long, but 33 for 25 us where 32 rows have 1500
 // positions. Two stages and five CTAs instead of three and four: 62 -> 50 us at the first; Q in shared memory,
 // not registers: 50 -> 46.
 #include <algorithm>
@@ -244,29 +244,40 @@ __device__ __forceinline__ void few_rows(const AttendTreeArgs &a, const FewItem 
         }
     }
     const auto values = [&](auto clean) {
+      uint32_t ph[NT / 2][4], pl[NT / 2][4];
 #pragma unroll
-      for (int kk = 0; kk < NT / 2; ++kk) {
-        uint32_t ph[4], pl[4];
+      for (int kk = 0; kk < NT / 2; ++kk)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const float p = sc[2 * kk + (x >> 1)][2 * (x & 1)], q = sc[2 * kk + (x >> 1)][2 * (x & 1) + 1];
-          if constexpr (WIDE) split2(p, q, ph[x], pl[x]);
-          else ph[x] = pack_half2(p, q);
+          if constexpr (WIDE) split2(p, q, ph[kk][x], pl[kk][x]);
+          else ph[kk][x] = pack_half2(p, q);
         }
 #pragma unroll
-        for (int n = 0; n < KS; ++n) {
+      for (int n = 0; n < KS; ++n) {
+        // f32: a tile's products apart from the sums over the tiles, which f32 additions round: a step of a
+        // tensor-core sum drops bits of its size.
+        float part[2][4] = {};
+#pragma unroll
+        for (int kk = 0; kk < NT / 2; ++kk) {
           uint32_t b[4];
           ldsm4_t(b, vb + tile_at(first + kk * 16 + (lane & 15), 2 * n + (lane >> 4)));
           if constexpr (decltype(clean)::value)
 #pragma unroll
             for (int x = 0; x < 4; ++x) b[x] = finite2(b[x]);
-          mma16(acc[2 * n], ph, b[0], b[1]);
-          mma16(acc[2 * n + 1], ph, b[2], b[3]);
           if constexpr (WIDE) {
-            mma16(acc[2 * n], pl, b[0], b[1]);
-            mma16(acc[2 * n + 1], pl, b[2], b[3]);
+            mma16(part[0], pl[kk], b[0], b[1]);
+            mma16(part[1], pl[kk], b[2], b[3]);
+            mma16(part[0], ph[kk], b[0], b[1]);
+            mma16(part[1], ph[kk], b[2], b[3]);
+          } else {
+            mma16(acc[2 * n], ph[kk], b[0], b[1]);
+            mma16(acc[2 * n + 1], ph[kk], b[2], b[3]);
           }
         }
+        if constexpr (WIDE)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) acc[2 * n + (x >> 2)][x & 3] += part[x >> 2][x & 3];
       }
     };
     if (!odd) {
