@@ -1,9 +1,9 @@
-// Paged KV caches: the plan of a step (block tables and slot maps from request lengths) and the write
-// of its K and V rows.
+// Paged KV caches: the plan of a step (block tables and slot maps from request lengths) and the
+// write of its K and V rows.
 //
 // A cache ("pool") is f16 [blocks][K, V][kv_heads][bs][hd]: the bs positions of one head's K (or V)
-// in a block are one contiguous tile of bs x hd, which the attention loads as rows of a matrix. A slot
-// is block * bs + offset.
+// in a block are one contiguous tile of bs x hd, which the attention loads as rows of a matrix. A
+// slot is block * bs + offset.
 #include <algorithm>
 
 #include "kernels.cuh"
@@ -19,11 +19,11 @@ namespace {
 // sum only grows, so the granted requests' blocks are one run of the ring of free blocks from its
 // head; what finished requests give back goes behind its tail, which no request of this call reads.
 //
-// One launch and no hand-over between CTAs: a CTA takes `per` consecutive requests, sums what
-// the others before it need (and what all do) from the 12 bytes of each, and scans its own. A few
-// microseconds of latency, not bytes, bound it: at 2048 requests every CTA reads 24 KB out of L2. 32 requests
-// of 16 rows take 6.7 us on the device from cold caches, 2048 requests of up to 96 rows 16 us; a call from
-// Python costs the host 8 to 10 us.
+// One launch and no hand-over between CTAs: a CTA takes `per` consecutive requests, sums what the
+// others before it need (and what all do) from the 12 bytes of each, and scans its own. A few
+// microseconds of latency, not bytes, bound it: at 2048 requests every CTA reads 24 KB out of L2.
+// 32 requests of 16 rows take 6.7 us on the device from cold caches, 2048 requests of up to 96 rows
+// 16 us; a call from Python costs the host 8 to 10 us.
 constexpr int BT_THREADS = 256;
 
 struct BtNeed {
@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(BT_THREADS) block_tables_kernel(const BlockTab
 // ---- K and V rows into the cache ----------------------------------------------------------
 
 // Eight elements a thread and row (one 16-byte store); a thread keeps its place in the row, so that
-// the head and the element are divided out once. Bound by the memory: 48000 f32 rows of 2560 (737 MB)
-// take 126 us, 5.9 TB/s, 0.91 of the measured copy.
+// the head and the element are divided out once. Bound by the memory: 48000 f32 rows of 2560 (737
+// MB) take 126 us, 5.9 TB/s, 0.91 of the measured copy.
 template <typename T, bool VEC>
 __device__ __forceinline__ uint4 load8(const T *p) {
   uint4 o;
@@ -267,10 +267,10 @@ __global__ void __launch_bounds__(256)
 // test is one comparison of mask words. Warp 0 walks (32 candidates a step); every layer's CTA
 // walks for itself, which costs less than a second launch. Then the accepted nodes' K and V move to
 // consecutive positions. path[k] >= k and rises, so no destination is the source of a later move,
-// and a thread that keeps its place in the head and walks k upwards needs no barrier.
-// A chain of latencies (row starts, tokens, the walk, table entries, one load and store) bounds it: 128
-// requests of up to 64 nodes over 4 layers take 9 to 12 us on the device from cold caches, and took 16 to 20
-// with each move's store before the next move's load.
+// and a thread that keeps its place in the head and walks k upwards needs no barrier. A chain of
+// latencies (row starts, tokens, the walk, table entries, one load and store) bounds it: 128
+// requests of up to 64 nodes over 4 layers take 9 to 12 us on the device from cold caches, and took
+// 16 to 20 with each move's store before the next move's load.
 constexpr int TA_THREADS = 256;
 constexpr int TA_MAX = 256;  // nodes of a tree
 constexpr int TA_BATCH = 8;
@@ -280,7 +280,8 @@ __global__ void __launch_bounds__(TA_THREADS) tree_accept_kernel(const TreeAccep
   griddep_wait();  // the previous kernel of the stream has completed (programmatic launch)
   __shared__ uint32_t mask[TA_MAX * 8];
   __shared__ int tok[TA_MAX], pick[TA_MAX], path[TA_MAX];
-  // Element offsets of the accepted nodes off their place, and of the places they go to; -1: not there.
+  // Element offsets of the accepted nodes off their place, and of the places they go to; -1: not
+  // there.
   __shared__ long long from[TA_MAX], to[TA_MAX];
   __shared__ int s_count;
   const int s = int(blockIdx.x), layer = int(blockIdx.y), tid = int(threadIdx.x);

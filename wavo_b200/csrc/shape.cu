@@ -9,17 +9,17 @@ namespace wv {
 namespace {
 
 // A row's vocabulary is cut into ranges, one a CTA; the CTAs of a row form a cluster (8 at most). A
-// range passes through registers, four tokens a load and the next ones on their way: read once, masked,
-// written where it is wanted, and reduced to (maximum, its first index, sum of exponentials), which
-// meets the other CTAs' through distributed shared memory.
-// The tokens that a row's history, path or biases name are few, and their edits (a division among
-// them) many times the work of the others'. A bit a token takes them out of that pass; in the order of
-// their ids they have a place each in a list, with a word: how often the token is in the history and
-// the path in the low half, 1 + the last entry of its bias in the high half (whole numbers, so the
-// order of the atomics does not matter). A thread edits one of them.
-// 249 rows of 51866 f32 logits with grammars, 448 tokens of history and 200 biases (105 MB read and
-// written): 30 us, 3.5 TB/s; about half the issue slots are taken and 249 rows leave 47 of the 148 SMs with
-// one row where the others have two. 32 rows 10 us, the call's host side.
+// range passes through registers, four tokens a load and the next ones on their way: read once,
+// masked, written where it is wanted, and reduced to (maximum, its first index, sum of
+// exponentials), which meets the other CTAs' through distributed shared memory. The tokens that a
+// row's history, path or biases name are few, and their edits (a division among them) many times
+// the work of the others'. A bit a token takes them out of that pass; in the order of their ids
+// they have a place each in a list, with a word: how often the token is in the history and the path
+// in the low half, 1 + the last entry of its bias in the high half (whole numbers, so the order of
+// the atomics does not matter). A thread edits one of them. 249 rows of 51866 f32 logits with
+// grammars, 448 tokens of history and 200 biases (105 MB read and written): 30 us, 3.5 TB/s; about
+// half the issue slots are taken and 249 rows leave 47 of the 148 SMs with one row where the others
+// have two. 32 rows 10 us, the call's host side.
 constexpr int SH_THREADS = 512;
 constexpr int SH_WARPS = SH_THREADS / 32;
 constexpr int SH_G = 2;                         // groups of four tokens a thread holds
@@ -318,8 +318,8 @@ __global__ void __launch_bounds__(SH_THREADS, 2)
 template <typename T>
 cudaError_t launch(const ShapeArgs &a, int sms, cudaStream_t s) {
   // As many CTAs a row (a power of two) as the SMs hold at once, two each; ranges of 2048 tokens at
-  // least. Every CTA names the row's tokens anew and waits for its cluster, so more cost more:
-  // 249 rows of 51866 with 1, 2, 4, 8 CTAs 30, 37, 51, 80 us, 90 rows 25, 19, 25, 32, 32 rows 17, 14,
+  // least. Every CTA names the row's tokens anew and waits for its cluster, so more cost more: 249
+  // rows of 51866 with 1, 2, 4, 8 CTAs 30, 37, 51, 80 us, 90 rows 25, 19, 25, 32, 32 rows 17, 14,
   // 12, 11.
   int ctas = 1;
   while (ctas < SH_CTAS && a.rows * 2ll * ctas <= 2ll * sms && a.vocab / (2 * ctas) >= 2048) ctas *= 2;

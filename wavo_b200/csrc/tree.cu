@@ -4,26 +4,26 @@
 // it whose bits its mask words hold (row j's K and V are at position len + j). o = softmax(q.k /
 // sqrt(hd)) v over what it sees, zeros where it sees nothing.
 //
-// This is the form for many rows (tree_few.cu has the one for few). One pass over K and V with a running
-// softmax. An item is one K and V head of one request with up to 128 rows that read it (its drafted rows
-// and the heads that share it); the rows are the UMMA's M and 128 positions its N,
+// This is the form for many rows (tree_few.cu has the one for few). One pass over K and V with a
+// running softmax. An item is one K and V head of one request with up to 128 rows that read it (its
+// drafted rows and the heads that share it); the rows are the UMMA's M and 128 positions its N,
 //   S [128 x 128] = Q [128 x hd] . K^T,   O [128 x hd] += P [128 x 128] . V,
-// S and O in tensor memory and P there over the S that it came from. Two threads of a warp have a row's
-// scores of a tile, so its maximum takes one shuffle, and warps without rows do nothing. A row's
-// reference value rises when a score is 8 (base 2) above it, at which a probability is still 256 in
-// f16: at an item's first tile and seldom after, so O is seldom rescaled.
+// S and O in tensor memory and P there over the S that it came from. Two threads of a warp have a
+// row's scores of a tile, so its maximum takes one shuffle, and warps without rows do nothing. A
+// row's reference value rises when a score is 8 (base 2) above it, at which a probability is still
+// 256 in f16: at an item's first tile and seldom after, so O is seldom rescaled.
 //
-// The items' tiles of 128 positions lie one after another and are cut into equal runs, one a CTA, as
-// many CTAs as are resident: ragged lengths, few long requests and many short ones fill the GPU alike,
-// and the loads run ahead across the items of a run. A run that ends inside an item leaves its part in
-// global memory, and a second kernel joins an item's parts in the order of the runs.
+// The items' tiles of 128 positions lie one after another and are cut into equal runs, one a CTA,
+// as many CTAs as are resident: ragged lengths, few long requests and many short ones fill the GPU
+// alike, and the loads run ahead across the items of a run. A run that ends inside an item leaves
+// its part in global memory, and a second kernel joins an item's parts in the order of the runs.
 //
-// Two requests of up to 131072 positions, 8 K and V heads of 128 and up to 96 rows each (685 MB, 53 GFLOP):
-// 143 us and 9 for the join, 4.8 TB/s; the loads alone, in the same runs, take 137 to 157. A tile costs the
-// softmax warps about 2300 cycles (the exponentials 770 of them) and its 64 KB an SM's share of the memory
-// 2800; at the clocks that the power limit leaves the two are close. Positions as the UMMA's M and the rows as
-// its N (P through shared memory, a vote of all warps a tile) took 215 us, the join by the last CTA alone 57
-// more.
+// Two requests of up to 131072 positions, 8 K and V heads of 128 and up to 96 rows each (685 MB, 53
+// GFLOP): 143 us and 9 for the join, 4.8 TB/s; the loads alone, in the same runs, take 137 to 157.
+// A tile costs the softmax warps about 2300 cycles (the exponentials 770 of them) and its 64 KB an
+// SM's share of the memory 2800; at the clocks that the power limit leaves the two are close.
+// Positions as the UMMA's M and the rows as its N (P through shared memory, a vote of all warps a
+// tile) took 215 us, the join by the last CTA alone 57 more.
 #include <algorithm>
 #include <type_traits>
 
@@ -60,7 +60,8 @@ constexpr int TT_THREADS = TT_SOFT + 96;                            // and loads
 // A run's share of an item.
 struct TreePiece {
   int s, kvh, r0, here;     // request, K and V head, first row, rows
-  int lo, rows, len, keys;  // the request's first row, its drafted rows, positions without and with them
+  int lo, rows;             // the request's first row, its drafted rows
+  int len, keys;            // its positions without and with them
   int tile0, tiles;         // tiles of the item
   int slot;                 // where a partial result goes; -1: the item is whole
 };
@@ -110,7 +111,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
   constexpr int D = T::kRing, SOFT = TT_SOFT;
   constexpr int W_LOAD = SOFT / 32, W_MMA = W_LOAD + 1, W_ROWS = W_LOAD + 2, WARPS = W_LOAD + 3;
   extern __shared__ uint8_t raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                              ~uintptr_t(1023));
   TreeShared &sh = *reinterpret_cast<TreeShared *>(smem + T::kOffBar);
   const int tid = int(threadIdx.x), lane = tid & 31, w = int(warp_id());
   const int group = a.heads / a.kv_heads;
@@ -489,8 +491,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
     const float scale = a.scale * 1.4426950408889634f;  // exponentials of base 2
     for (int k = 0, g = 0; g < n; ++k) {
       const int pc = k % TT_PIECES;
-      // Where a wait gives up, all warps leave together; inside an item they run on (later waits give
-      // up soon).
+      // Where a wait gives up, all warps leave together; inside an item they run on (later waits
+      // give up soon).
       bool ok = mbar_wait_warp(&sh.row_full[pc], (k / TT_PIECES) & 1, ab, kErrTimeoutConsumer);
       if (any(!ok)) break;
       const TreePiece &q = sh.piece[pc];
@@ -504,9 +506,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
         const bool all = info >> 31;  // every row sees the whole tile
         const int pos0 = (q.tile0 + i) * TT_KEYS;
         if (!all && tid < TT_KEYS) {
-          // What a row does not see must not reach it through 0 times infinity: V is zero past the end,
-          // and a drafted position's infinities and NaN are zeros here and added at the end to the
-          // rows that see them.
+          // What a row does not see must not reach it through 0 times infinity: V is zero past the
+          // end, and a drafted position's infinities and NaN are zeros here and added at the end to
+          // the rows that see them.
           const int p = g == n - 1 ? 2 * n - 1 : 2 * g + 2, pos = pos0 + tid, d = pos - q.len;
           mbar_wait_warp(&sh.full[p % D], (p / D) & 1, ab, kErrTimeoutConsumer);
           const bool there = pos < q.keys && ((info >> (tid / min(a.bs, TT_KEYS))) & 1u);
@@ -645,7 +647,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
         const long long at = good ? rows.out[row] : -1;
         if (q.slot >= 0 && at >= 0 && half == 0)
           *reinterpret_cast<float2 *>(a.part + at + a.hd) = make_float2(m, sum);
-        const bool vec = q.slot >= 0 || ((reinterpret_cast<uintptr_t>(a.o) | (a.o_stride * sizeof(E))) & 15u) == 0;
+        const bool vec =
+            ((reinterpret_cast<uintptr_t>(a.o) | (a.o_stride * sizeof(E))) & 15u) == 0;
 #pragma unroll 1
         for (int c = 0; c < HDP / 2; c += 16) {
           const int dim = half * (HDP / 2) + c;
@@ -712,8 +715,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
   if (w == W_MMA) tmem_dealloc(tmem, 512);
 }
 
-// The parts of an item joined: CTA (c, y) takes 8 of the rows of the item that run c begins, if that
-// run does not end it. Four elements a thread.
+// The parts of an item joined: CTA (c, y) takes 8 of the rows of the item that run c begins, if
+// that run does not end it. Four elements a thread.
 constexpr int TT_JOIN = 8;
 
 template <typename E>
@@ -789,10 +792,11 @@ cudaError_t launch_tile(const CUtensorMap &map, const AttendTreeArgs &a, int sms
 
 }  // namespace
 
-// Measured on both sides, us few : many, f16 and f32. Long: 2 x 16384 positions, heads of 128: 32 rows 38 : 38, 46 : 49;
-// 48 rows 47 : 40, 62 : 53; 96 rows 70 : 53, 90 : 73; heads of 64: 32 rows 43 : 53, 54 : 57; 48 rows 66 : 57, 99 : 65. 32 x
-// 1500, heads of 64: 48 rows 95 : 87, 116 : 120; 96 rows 135 : 102, 176 : 155. Short: 32 x 512, heads of 128: 64 rows
-// 42 : 50, 48 : 74; 128 rows 66 : 74, 93 : 96; 192 rows 117 : 76, 118 : 124; heads of 64: 96 rows 62 : 63, 72 : 149.
+// Measured on both sides, us few : many, f16 and f32. Long: 2 x 16384 positions, heads of 128: 32
+// rows 38 : 38, 46 : 49; 48 rows 47 : 40, 62 : 53; 96 rows 70 : 53, 90 : 73; heads of 64: 32 rows
+// 43 : 53, 54 : 57; 48 rows 66 : 57, 99 : 65. 32 x 1500, heads of 64: 48 rows 95 : 87, 116 : 120;
+// 96 rows 135 : 102, 176 : 155. Short: 32 x 512, heads of 128: 64 rows 42 : 50, 48 : 74; 128 rows
+// 66 : 74, 93 : 96; 192 rows 117 : 76, 118 : 124; heads of 64: 96 rows 62 : 63, 72 : 149.
 bool attend_tree_few(int max_rows, int max_len, int heads, int kv_heads) {
   const long long rows = (long long)max_rows * (heads / kv_heads);
   return rows <= 32 || (rows <= 128 && max_len < 1280);

@@ -1,22 +1,23 @@
-// attend_tree for few rows: an item is one K and V head of one request with the rows that read it (its
-// drafted rows and the heads that share it), 32 at most in a CTA. The steps from a tile's arrival to its
-// sums are then short and the tiles of a request few, so what counts is how many of them are under way
-// at once: mma.sync with everything in registers between the products, no tensor memory, no hand-over
-// between warps, and 2 to 5 CTAs an SM. The form with tcgen05 (tree.cu) takes over where the products
-// would bound it; the figures of both are beside the rule there.
+// attend_tree for few rows: an item is one K and V head of one request with the rows that read it
+// (its drafted rows and the heads that share it), 32 at most in a CTA. The steps from a tile's
+// arrival to its sums are then short and the tiles of a request few, so what counts is how many of
+// them are under way at once: mma.sync with everything in registers between the products, no tensor
+// memory, no hand-over between warps, and 2 to 5 CTAs an SM. The form with tcgen05 (tree.cu) takes
+// over where the products would bound it; the figures of both are beside the rule there.
 //
-// One pass over K and V with the softmax's running maximum and sum: a CTA takes an item's rows over a
-// range of positions. A producer warp loads 64 positions at a time, page by page, through TMA boxes
-// that follow the block table; four warps multiply, 16 rows each: they share a tile's positions, and meet in
-// shared memory at the end.
+// One pass over K and V with the softmax's running maximum and sum: a CTA takes an item's rows over
+// a range of positions. A producer warp loads 64 positions at a time, page by page, through TMA
+// boxes that follow the block table; four warps multiply, 16 rows each: they share a tile's
+// positions, and meet in shared memory at the end.
 //
-// Bound by the loads: 32 x 20 items of 16 rows over 1500 positions (246 MB, f16) take 46 us, 5.3 TB/s; the same
-// loads without the products took 54 us in CTAs of their own. One f32 row an item over 448 positions at
-// most (34 MB) 18 us, of which launch and the first page's way (row starts, table, K) are most. Up to 64 f32 rows an
-// item over 448 positions (two products each way) 47 us, bound by the latency of 16 warps an SM; 64 rows a CTA, a
-// page read once, took 7 more (three CTAs an SM), 16 rows a CTA as long, but 33 for 25 us where 32 rows have 1500
-// positions. Two stages and five CTAs instead of three and four: 62 -> 50 us at the first; Q in shared memory,
-// not registers: 50 -> 46.
+// Bound by the loads: 32 x 20 items of 16 rows over 1500 positions (246 MB, f16) take 46 us, 5.3
+// TB/s; the same loads without the products took 54 us in CTAs of their own. One f32 row an item
+// over 448 positions at most (34 MB) 18 us, of which launch and the first page's way (row starts,
+// table, K) are most. Up to 64 f32 rows an item over 448 positions (two products each way) 47 us,
+// bound by the latency of 16 warps an SM; 64 rows a CTA, a page read once, took 7 more (three CTAs
+// an SM), 16 rows a CTA as long, but 33 for 25 us where 32 rows have 1500 positions. Two stages and
+// five CTAs instead of three and four: 62 -> 50 us at the first; Q in shared memory, not registers:
+// 50 -> 46.
 #include <algorithm>
 #include <type_traits>
 
@@ -155,7 +156,8 @@ __device__ __forceinline__ void few_rows(const AttendTreeArgs &a, const FewItem 
     const int first = wk * KEYS;  // the warp's first position in the tile
     const int p0 = k0 + i * TF_KEYS + first;
     float sc[NT][4] = {};
-    // The low parts first: the sums are small until the high ones come, and so is what a step drops.
+    // The low parts first: the sums are small until the high ones come, and so is what a step
+    // drops.
 #pragma unroll
     for (int part = WIDE ? 1 : 0; part >= 0; --part)
 #pragma unroll
@@ -249,14 +251,15 @@ __device__ __forceinline__ void few_rows(const AttendTreeArgs &a, const FewItem 
       for (int kk = 0; kk < NT / 2; ++kk)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const float p = sc[2 * kk + (x >> 1)][2 * (x & 1)], q = sc[2 * kk + (x >> 1)][2 * (x & 1) + 1];
+          const float p = sc[2 * kk + (x >> 1)][2 * (x & 1)];
+          const float q = sc[2 * kk + (x >> 1)][2 * (x & 1) + 1];
           if constexpr (WIDE) split2(p, q, ph[kk][x], pl[kk][x]);
           else ph[kk][x] = pack_half2(p, q);
         }
 #pragma unroll
       for (int n = 0; n < KS; ++n) {
-        // f32: a tile's products apart from the sums over the tiles, which f32 additions round: a step of a
-        // tensor-core sum drops bits of its size.
+        // f32: a tile's products apart from the sums over the tiles, which f32 additions round: a
+        // step of a tensor-core sum drops bits of its size.
         float part[2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < NT / 2; ++kk) {
@@ -385,7 +388,8 @@ __global__ void __launch_bounds__(TF_THREADS, FewTile<HDP, MAXR, WIDE>::kCtas)
   using T = FewTile<HDP, MAXR, WIDE>;
   constexpr int ST = T::kStages;
   extern __shared__ uint8_t raw[];
-  uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                               ~uintptr_t(1023));
   __shared__ FewShared<ST> sh;
   const int tid = int(threadIdx.x), lane = tid & 31, w = int(warp_id());
   const Abort ab{&sh.abort, a.err};
@@ -516,8 +520,8 @@ cudaError_t launch_few(const CUtensorMap &map, const AttendTreeArgs &a, cudaStre
 
 template <int HDP, bool WIDE>
 cudaError_t launch_rows(const CUtensorMap &map, const AttendTreeArgs &a, cudaStream_t s) {
-  return (long long)a.max_rows * (a.heads / a.kv_heads) <= 16 ? launch_few<HDP, 16, WIDE>(map, a, s)
-                                                              : launch_few<HDP, TF_ROWS, WIDE>(map, a, s);
+  const long long rows = (long long)a.max_rows * (a.heads / a.kv_heads);
+  return rows <= 16 ? launch_few<HDP, 16, WIDE>(map, a, s) : launch_few<HDP, TF_ROWS, WIDE>(map, a, s);
 }
 
 }  // namespace
