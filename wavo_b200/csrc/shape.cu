@@ -219,7 +219,6 @@ __global__ void __launch_bounds__(SH_THREADS, 2)
         if (e >> 16) z += a.bias_vals[(long long)s * a.max_bias + (e >> 16) - 1];
         if (allow && !((allow[i >> 5] >> (i & 31)) & 1u)) z = -INFINITY;
         sh.note[k] = __float_as_uint(z);
-        shape_join(all, z, z == -INFINITY ? 0.0f : isnan(z) ? z : 1.0f, i);
       }
       if (out == in) __syncthreads();  // the pass writes over what was read here
     }
@@ -281,9 +280,14 @@ __global__ void __launch_bounds__(SH_THREADS, 2)
     }
     if (listed) {
       __syncthreads();  // the pass has written its values there
-      if (out)
-        for (int k = tid; k < listed; k += SH_THREADS)
-          out[sh.list[k] + lo - shift] = T(__uint_as_float(sh.note[k]));
+      // The named tokens join the maximum here: the pass takes the first of equal values by going
+      // upwards, and these are below and above what it has seen.
+      for (int k = tid; k < listed; k += SH_THREADS) {
+        const int i = sh.list[k] + lo - shift;
+        const float z = __uint_as_float(sh.note[k]);
+        if (out) out[i] = T(z);
+        shape_join(all, z, z == -INFINITY ? 0.0f : isnan(z) ? z : 1.0f, i);
+      }
     }
     if (any_named && hi < end) __syncthreads();  // the list is made anew
   }
