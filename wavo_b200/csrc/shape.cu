@@ -268,15 +268,17 @@ __global__ void __launch_bounds__(SH_THREADS, 2)
           }
         }
       }
-      const float base = top == -INFINITY ? 0.0f : top * SH_LOG2E;
+      // The difference first: a rounded product of the maximum would be common to all terms and stay
+      // in the sum, and past the largest value it is no number.
+      const float base = top == -INFINITY ? 0.0f : top;
       if (top > all.top) {
-        all.sum *= ex2(fmaf(all.top, SH_LOG2E, -base));
+        all.sum *= ex2((all.top - base) * SH_LOG2E);
         all.top = top;
       }
 #pragma unroll
       for (int j = 0; j < SH_G; ++j)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) all.sum += ex2(fmaf(x[j][y], SH_LOG2E, -base));
+        for (int y = 0; y < 4; ++y) all.sum += ex2((x[j][y] - base) * SH_LOG2E);
     }
     if (listed) {
       __syncthreads();  // the pass has written its values there
