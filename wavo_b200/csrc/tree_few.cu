@@ -218,14 +218,16 @@ __device__ __forceinline__ void few_rows(const AttendTreeArgs &a, const FewItem 
         odd = __any_sync(0xffffffffu, bad);
       }
     }
-    // The running maximum and sum, two rows a thread (four threads a row).
+    // The running reference and sum, two rows a thread (four threads a row). The reference is the
+    // maximum, or kLift below it, rounded up, so that no probability passes 1, or 2^kLift.
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      float mx = m[u];
+      float mx = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * u], sc[n][2 * u + 1]) * scale);
+      for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * u], sc[n][2 * u + 1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      mx = fmaxf(m[u], __fmaf_ru(mx, scale, WIDE ? 0.0f : -float(kLift)));
       const float base = mx == -INFINITY ? 0.0f : mx;
       const float carry = ex2(m[u] - base);
       m[u] = mx;
@@ -253,34 +255,40 @@ __device__ __forceinline__ void few_rows(const AttendTreeArgs &a, const FewItem 
         for (int x = 0; x < 4; ++x) {
           const float p = sc[2 * kk + (x >> 1)][2 * (x & 1)];
           const float q = sc[2 * kk + (x >> 1)][2 * (x & 1) + 1];
-          if constexpr (WIDE) split2(p, q, ph[kk][x], pl[kk][x]);
+          if constexpr (WIDE) split2_up<kLift>(p, q, ph[kk][x], pl[kk][x]);
           else ph[kk][x] = pack_half2(p, q);
         }
 #pragma unroll
       for (int n = 0; n < KS; ++n) {
         // f32: a tile's products apart from the sums over the tiles, which f32 additions round: a
-        // step of a tensor-core sum drops bits of its size.
+        // step of a tensor-core sum drops bits of its size. The low parts' first, scaled back.
         float part[2][4] = {};
+        uint32_t b[NT / 2][4];
 #pragma unroll
         for (int kk = 0; kk < NT / 2; ++kk) {
-          uint32_t b[4];
-          ldsm4_t(b, vb + tile_at(first + kk * 16 + (lane & 15), 2 * n + (lane >> 4)));
+          ldsm4_t(b[kk], vb + tile_at(first + kk * 16 + (lane & 15), 2 * n + (lane >> 4)));
           if constexpr (decltype(clean)::value)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) b[x] = finite2(b[x]);
+            for (int x = 0; x < 4; ++x) b[kk][x] = finite2(b[kk][x]);
           if constexpr (WIDE) {
-            mma16(part[0], pl[kk], b[0], b[1]);
-            mma16(part[1], pl[kk], b[2], b[3]);
-            mma16(part[0], ph[kk], b[0], b[1]);
-            mma16(part[1], ph[kk], b[2], b[3]);
+            mma16(part[0], pl[kk], b[kk][0], b[kk][1]);
+            mma16(part[1], pl[kk], b[kk][2], b[kk][3]);
           } else {
-            mma16(acc[2 * n], ph[kk], b[0], b[1]);
-            mma16(acc[2 * n + 1], ph[kk], b[2], b[3]);
+            mma16(acc[2 * n], ph[kk], b[kk][0], b[kk][1]);
+            mma16(acc[2 * n + 1], ph[kk], b[kk][2], b[kk][3]);
           }
         }
-        if constexpr (WIDE)
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) part[x >> 2][x & 3] *= 1.0f / kLowUp;
+#pragma unroll
+          for (int kk = 0; kk < NT / 2; ++kk) {
+            mma16(part[0], ph[kk], b[kk][0], b[kk][1]);
+            mma16(part[1], ph[kk], b[kk][2], b[kk][3]);
+          }
 #pragma unroll
           for (int x = 0; x < 8; ++x) acc[2 * n + (x >> 2)][x & 3] += part[x >> 2][x & 3];
+        }
       }
     };
     if (!odd) {
@@ -363,11 +371,12 @@ __device__ __forceinline__ void few_rows(const AttendTreeArgs &a, const FewItem 
     for (int k = 0; k < WK; ++k) {
       const float x = ex2(sh.m[k * WR + (r >> 4)][r & 15] - base);
       const float4 v = *reinterpret_cast<const float4 *>(sum + (k * MT + r) * HDP + c);
+      const float y = WIDE ? x * (1.0f / (1 << kLift)) : x;
       total = fmaf(x, sh.l[k * WR + (r >> 4)][r & 15], total);
-      o[0] = fmaf(x, v.x, o[0]);
-      o[1] = fmaf(x, v.y, o[1]);
-      o[2] = fmaf(x, v.z, o[2]);
-      o[3] = fmaf(x, v.w, o[3]);
+      o[0] = fmaf(y, v.x, o[0]);
+      o[1] = fmaf(y, v.y, o[1]);
+      o[2] = fmaf(y, v.z, o[2]);
+      o[3] = fmaf(y, v.w, o[3]);
     }
     if (a.splits == 1) {
       const float inv = total != 0.0f ? 1.0f / total : 0.0f;
