@@ -48,6 +48,7 @@ struct TreeTile {
   static constexpr uint32_t kQ = (HDP / 64) * TT_HALF;              // Q, one part
   static constexpr int kQBufs = kParts * kQ > 16384 ? 1 : 2;
   static constexpr int kRing = HDP == 64 ? 8 : WIDE ? 4 : 5;
+  static_assert(kRing >= 4, "the softmax's wait for V");
   static constexpr uint32_t kOffQ = kRing * kSlot;
   static constexpr uint32_t kOffBar = kOffQ + kQBufs * kParts * kQ;
   // TMEM: S and P twice, then O; f32's low parts sum apart (each step of a long sum drops bits of
@@ -505,10 +506,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
         const uint32_t info = sh.info[g & 7];
         const bool all = info >> 31;  // every row sees the whole tile
         const int pos0 = (q.tile0 + i) * TT_KEYS;
+        mbar_wait_warp(&sh.s_full[g & 1], (g >> 1) & 1, ab, kErrTimeoutConsumer);
+        tc_fence_after();
         if (!all && tid < TT_KEYS) {
           // What a row does not see must not reach it through 0 times infinity: V is zero past the
           // end, and a drafted position's infinities and NaN are zeros here and added at the end to
-          // the rows that see them.
+          // the rows that see them. (After S of this tile, and so after P.V of two tiles before: in a
+          // ring of four that V lies in this one's place, and a wait by parity that starts before it
+          // has landed is let through at once.)
           const int p = g == n - 1 ? 2 * n - 1 : 2 * g + 2, pos = pos0 + tid, d = pos - q.len;
           mbar_wait_warp(&sh.full[p % D], (p / D) & 1, ab, kErrTimeoutConsumer);
           const bool there = pos < q.keys && ((info >> (tid / min(a.bs, TT_KEYS))) & 1u);
@@ -530,8 +535,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
           }
           fence_proxy_async_smem();
         }
-        mbar_wait_warp(&sh.s_full[g & 1], (g >> 1) & 1, ab, kErrTimeoutConsumer);
-        tc_fence_after();
         if (work) {
           float x[64];
           {
