@@ -385,10 +385,11 @@ wavo_status wavo_pack_slots(wavo_ctx *ctx, const void *x, int x_dtype, uint32_t 
  * 32 * mask_words with a mask), max_len at least every number of positions, cached and drafted
  * (what lies beyond is not seen). Scores are scaled by 1 / sqrt(hd). A row that sees nothing gets
  * zeros; what a row does not see has no effect on it, whatever it holds. WAVO_F16: f16 products,
- * f32 sums, probabilities rounded to f16 before they meet V. WAVO_F32: q and the probabilities enter
- * as two f16 parts each, for f32 accuracy (q below f16's largest value; measured against 64 bits:
- * relative 2-norms of 2e-7 to 3e-6, growing with the positions). Table entries outside the pool
- * are positions that no row sees.
+ * f32 sums, probabilities rounded to f16 before they meet V (to 2^-11 of each, down to 2^-25 of the
+ * row's largest). WAVO_F32: q and the probabilities enter as two f16 parts each, for f32 accuracy:
+ * the probabilities to 2^-22 of each down to the same 2^-25, q (below f16's largest value) to 2^-22
+ * or 2^-25, whichever is more. Measured against 64 bits: relative 2-norms of 2e-7 to 3e-6, growing
+ * with the positions. Table entries outside the pool are positions that no row sees.
  * wavo_attend_tree_scratch is the scratch that a call needs (see wavo_reserve). */
 wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, int dtype,
                              const void *pool, uint32_t blocks, uint32_t bs, const int32_t *table,

@@ -91,3 +91,27 @@ def test_a_sink_few_rows_sizes(gpu, dtype, gap, hd, n, at):
     got, want, terms = sink_case(gpu, dtype, gap, at, n, 20, 2, 2, hd, 1, False)
     lim = bound(want, terms, dtype == "f16", 2.0 ** -40 if dtype == "f16" else 2.0 ** -50)
     assert (np.abs(got - want) <= lim).all(), (np.abs(got - want) / lim).max()
+
+
+# The kernel for many rows (more than 128 of a K and V head, or more than 32 over a long cache).
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("gap", [10, 12, 15, 18])
+@pytest.mark.parametrize("where", ["first", "middle", "last", "drafted"])
+@pytest.mark.parametrize("mean", [0, 1])
+def test_a_sink_many_rows(gpu, dtype, gap, where, mean):
+    n, t = 300, 20
+    at = {"first": 0, "middle": 150, "last": n - 1, "drafted": n + 2}[where]
+    got, want, terms = sink_case(gpu, dtype, gap, at, n, t, 16, 2, 64, mean, where == "drafted")
+    # The largest probability is 2^7 to 2^15 where it is rounded.
+    lim = bound(want, terms, dtype == "f16", 2.0 ** -32 if dtype == "f16" else 2.0 ** -42)
+    assert (np.abs(got - want) <= lim).all(), (np.abs(got - want) / lim).max()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("gap", [12, 18])
+@pytest.mark.parametrize("hd,n,at", [(64, 1, 0), (128, 4000, 40), (40, 1500, 1499), (64, 4000, 2000)])
+def test_a_sink_many_rows_sizes(gpu, dtype, gap, hd, n, at):
+    got, want, terms = sink_case(gpu, dtype, gap, at, n, 17, 8, 1, hd, 1, False)
+    lim = bound(want, terms, dtype == "f16", 2.0 ** -32 if dtype == "f16" else 2.0 ** -42)
+    assert (np.abs(got - want) <= lim).all(), (np.abs(got - want) / lim).max()

@@ -10,8 +10,9 @@
 //   S [128 x 128] = Q [128 x hd] . K^T,   O [128 x hd] += P [128 x 128] . V,
 // S and O in tensor memory and P there over the S that it came from. Two threads of a warp have a
 // row's scores of a tile, so its maximum takes one shuffle, and warps without rows do nothing. A
-// row's reference value rises when a score is 8 (base 2) above it, at which a probability is still
-// 256 in f16: at an item's first tile and seldom after, so O is seldom rescaled.
+// row's reference value rises when a score is 4 (base 2) above the one that set it: at an item's
+// first tile and seldom after, so O is seldom rescaled. The largest probability is then 2^11 to 2^15
+// where it is rounded to f16 (see kLift).
 //
 // The items' tiles of 128 positions lie one after another and are cut into equal runs, one a CTA,
 // as many CTAs as are resident: ragged lengths, few long requests and many short ones fill the GPU
@@ -36,7 +37,8 @@ namespace {
 constexpr int TT_KEYS = 128;                  // positions a tile
 constexpr uint32_t TT_HALF = TT_KEYS * 128;   // bytes of 128 positions x 64 elements
 constexpr int TT_ROWS = 128;                  // rows of an item
-constexpr float TT_RISE = 8.0f;
+constexpr int TT_RISE = 4;
+constexpr int TT_LIFT = kLift - TT_RISE;      // log2 of the probability of a reference
 constexpr int TT_PIECES = 3;                  // items in flight: loaded, multiplied, written
 constexpr int TT_WHOLE = 4;                   // items of up to this many tiles stay in one run
 
@@ -51,8 +53,8 @@ struct TreeTile {
   static_assert(kRing >= 4, "the softmax's wait for V");
   static constexpr uint32_t kOffQ = kRing * kSlot;
   static constexpr uint32_t kOffBar = kOffQ + kQBufs * kParts * kQ;
-  // TMEM: S and P twice, then O; f32's low parts sum apart (each step of a long sum drops bits of
-  // its size), and join at the end.
+  // TMEM: S and P twice, then O; f32's low parts sum apart (they are scaled, and each step of a long
+  // sum drops bits of its size), and join at the end.
   static constexpr uint32_t kColO = 256;
 };
 constexpr int TT_SOFT = 256;                                        // softmax threads
@@ -580,9 +582,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
               t = max3(t, x[y + 6], x[y + 7]);
             }
             top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) * scale;
+            // The reference it would set, rounded up: what it stands for is at most 2^TT_LIFT.
+            top = __fmaf_ru(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), scale,
+                            WIDE ? 0.0f : -float(TT_LIFT));
           }
-          const bool rise = top > m + TT_RISE;  // (-inf + 8 at the first score)
+          const bool rise = top > __fadd_rd(m, float(TT_RISE));  // (-inf + 4 at the first score)
           const float fac = rise ? ex2(m - top) : 1.0f;
           if (__any_sync(0xffffffffu, rise)) {
             l0 *= fac;
@@ -625,7 +629,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
           if constexpr (WIDE) {
             uint32_t low[32];
 #pragma unroll
-            for (int y = 0; y < 32; ++y) split2(x[2 * y], x[2 * y + 1], hi[y], low[y]);
+            for (int y = 0; y < 32; ++y) split2_up<TT_LIFT>(x[2 * y], x[2 * y + 1], hi[y], low[y]);
             tmem_st_16x2_x32<32>(lanes + (g & 1) * 128 + 64, low);
           }
           tmem_st_16x2_x32<32>(lanes + (g & 1) * 128, hi);
@@ -666,7 +670,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
             tmem_ld_16x2_x16<HDP / 2>(lanes + T::kColO + HDP + c, u);
             tmem_wait_ld();
 #pragma unroll
-            for (int y = 0; y < 16; ++y) o[y] += __uint_as_float(u[y]);
+            for (int y = 0; y < 16; ++y)
+              o[y] = fmaf(__uint_as_float(u[y]), 1.0f / kLowUp, o[y]) * (1.0f / (1 << TT_LIFT));
           }
           if (odd && at >= 0) {
             const int *table = a.table + (long long)q.s * a.width;
