@@ -355,8 +355,10 @@ wavo_status wavo_pick(wavo_ctx *ctx, float *logits, uint32_t ld, uint32_t rows, 
  * is done and gives its blocks back. Free block ids are a ring of ring_cap ids, state[0] the index of
  * the first, state[1] how many. Requests take the blocks they lack, in order, while they last: a
  * request is refused when the blocks lacking up to and with its own exceed those free, or when it
- * needs more than `width`; it then keeps what it has and its rows get no slots. A request that
- * lacks none is always served. Blocks given back can be taken from the next call on.
+ * needs more than `width`; it then keeps what it has, its rows get no slots, and the entries of its
+ * table for the blocks that it lacks become -1 where they named one (the attention sees and the
+ * commit moves nothing there). A request that lacks none is always served. Blocks given back can be
+ * taken from the next call on.
  * Out: the tables' new entries; owned_out; row_start [n + 1] (all requests' rows, refused ones'
  * too); for rows below rows_cap row_seq (the request) and slots, both -1 past the last row, slots
  * -1 for refused requests; state_out: the ring's new state, the number of rows, the number of
@@ -445,7 +447,8 @@ wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint
  * far as that goes. path [n][max_rows] gets the nodes, then -1; count [n] how many (0 for a request
  * without rows); next [n] the last node's pick (-1 without rows); new_lens[s] = lens[s] + count (not
  * the same buffer as lens: EINVAL). With a pool of `layers` layers, layer_stride elements apart, the
- * K and V of node path[k] move to position lens[s] + k in each. max_rows <= 256, mask_words <= 8. */
+ * K and V of node path[k] move to position lens[s] + k in each; nothing moves from or to a place whose
+ * table entry names no block (a refused request's). max_rows <= 256, mask_words <= 8. */
 wavo_status wavo_tree_accept(wavo_ctx *ctx, const int32_t *picks, const int32_t *tokens,
                              const uint32_t *mask, uint32_t mask_words, uint32_t rows,
                              const int32_t *row_start, uint32_t n, uint32_t max_rows,

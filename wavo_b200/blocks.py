@@ -614,9 +614,9 @@ class TreeDecoder:
         if rows == 0:
             return [[] for _ in trees]
         self._record(p, rows, most)
+        self._refused()  # before the commit, so that the caches are those of the step before
         p.tree_accept(self.picks, self.tokens[:rows], self.mask[:rows], self.row_start, self.lens,
                       self.table, self.pool, self.path, self.count, self.next, self.lens_next)
-        self._refused()
         out = torch.cat([self.path, self.count[:, None], self.next[:, None]], 1).tolist()
         self._keep(self.count, self.row_start[:-1, None] + self.path)
         gained = []

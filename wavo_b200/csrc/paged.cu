@@ -18,6 +18,9 @@ namespace {
 // while they fit: granted iff need = 0 or the running sum of needs (itself included) <= free. The
 // sum only grows, so the granted requests' blocks are one run of the ring of free blocks from its
 // head; what finished requests give back goes behind its tail, which no request of this call reads.
+// A refused request's entries for the blocks that it lacks may name blocks of others (zeros from the
+// start, or what it gave back once): they become -1, so that neither the attention nor the commit of
+// the same step reaches those blocks through its rows.
 //
 // One launch and no hand-over between CTAs: a CTA takes `per` consecutive requests, sums what the
 // others before it need (and what all do) from the 12 bytes of each, and scans its own. A few
@@ -76,7 +79,7 @@ __global__ void __launch_bounds__(BT_THREADS) block_tables_kernel(const BlockTab
   __shared__ int scan_i[W];
   __shared__ long long first[BT_THREADS + 1];  // first row of each request of this CTA
   __shared__ int s_len[BT_THREADS], s_owned[BT_THREADS], s_at[BT_THREADS], s_got[BT_THREADS],
-      s_gone[BT_THREADS], s_back[BT_THREADS];
+      s_gone[BT_THREADS], s_back[BT_THREADS], s_lack[BT_THREADS];
   __shared__ bool s_ok[BT_THREADS];
   const int tid = int(threadIdx.x), lane = tid & 31, w = tid >> 5;
   const int lo = int(blockIdx.x) * per, hi = min(a.n, lo + per);
@@ -144,6 +147,7 @@ __global__ void __launch_bounds__(BT_THREADS) block_tables_kernel(const BlockTab
     s_got[tid] = got;
     s_ok[tid] = ok;
     s_gone[tid] = r.gone;
+    s_lack[tid] = ok || back ? 0 : r.wide ? a.width - r.owned : r.need;
     s_back[tid] = int((head + (long long)free + gone_end - r.gone) % a.cap);
     if (writer) {
       a.row_start[s + 1] = int(min(row_end, 0x7fffffffll));
@@ -175,6 +179,8 @@ __global__ void __launch_bounds__(BT_THREADS) block_tables_kernel(const BlockTab
         t[s_owned[q] + k] = a.ring[int((s_at[q] + (long long)k) % a.cap)];
       for (int k = lane; k < s_gone[q]; k += 32)
         a.ring[int((s_back[q] + (long long)k) % a.cap)] = t[k];
+      for (int k = lane; k < s_lack[q]; k += 32)
+        if (t[s_owned[q] + k] >= 0) t[s_owned[q] + k] = -1;
     }
   }
   // Slots of this CTA's rows; a block taken in this call is read from the ring.
