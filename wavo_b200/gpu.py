@@ -52,6 +52,15 @@ def _f32(t) -> int:
     raise TypeError("contiguous float32 buffers on the GPU")
 
 
+def _row_stride(t: torch.Tensor, rows: int, wide: int) -> int:
+    """Elements from a row of t [rows][wide at least] to the next, as the ABI takes it (where 0 stands
+    for dense rows)."""
+    row, el = t.stride()
+    if el != 1 and wide > 1 or rows > 1 and row < wide:
+        raise ValueError(f"rows of {wide} elements with strides {(row, el)}")
+    return row if rows > 1 else wide
+
+
 def _pool(pool: torch.Tensor, dims: int = 5):
     """The address, blocks, kv_heads, bs and hd of a paged cache ([layers]) [blocks][2][kv_heads][bs][hd]
     in f16."""
@@ -470,7 +479,6 @@ class Pass:
         cache, blocks, kv_heads, bs, hd = _pool(pool)
         rows, wide = q.shape
         n, width = table.shape
-        (q_row, q_el), (o_row, o_el) = q.stride(), o.stride()
         starts = bits = None
         words = 0
         if row_start is not None:
@@ -482,9 +490,10 @@ class Pass:
             held, words = mask.shape
             if held < rows:
                 raise ValueError("attend_tree: the mask has fewer rows")
-        if q_el != 1 or o_el != 1 or o.shape != q.shape or o.dtype is not q.dtype or wide % hd or \
+        if o.shape != q.shape or o.dtype is not q.dtype or wide % hd or \
                 lens.numel() != n:
             raise ValueError("attend_tree: sizes or types differ")
+        q_row, o_row = _row_stride(q, rows, wide), _row_stride(o, rows, wide)
         status = L.lib().wavo_attend_tree(
             self.ctx, _ptr(q), q_row, _dtype(q), cache, blocks, bs, _i32(table), width, starts,
             _i32(lens), n, bits, words, rows, max_rows, max_len, _ptr(o), o_row, wide // hd, kv_heads,
@@ -497,19 +506,18 @@ class Pass:
         """The logits [rows][vocab] edited by the rules into out (None: not wanted; may be logits),
         their first maximum and its log-softmax (wavo_shape_logits)."""
         rows, wide = logits.shape
-        ld, step = logits.stride()
         vocab = rules.c.vocab
         to, ld_out = None, 0
         if out is not None:
-            ld_out, out_step = out.stride()
-            if out_step != 1 or out.dtype is not logits.dtype or out.shape[0] < rows or \
+            if out.dtype is not logits.dtype or out.shape[0] < rows or \
                     out.shape[1] < vocab:
                 raise ValueError("shape_logits: sizes or types of out differ")
-            to = _ptr(out)
-        if step != 1 or wide < vocab or rules.most < rows or \
+            to, ld_out = _ptr(out), _row_stride(out, rows, vocab)
+        if wide < vocab or rules.most < rows or \
                 (picks is not None and picks.numel() < rows) or \
                 (logprobs is not None and logprobs.numel() < rows):
             raise ValueError("shape_logits: sizes differ")
+        ld = _row_stride(logits, rows, vocab)
         status = L.lib().wavo_shape_logits(
             self.ctx, _ptr(logits), _dtype(logits), ld, to, ld_out, rows, rules.ref,
             None if picks is None else _i32(picks), None if logprobs is None else _f32(logprobs))
