@@ -64,3 +64,23 @@ def test_logits_that_share_memory_between_rows(gpu):
                    out=out.as_strided((1, 100), (2, 1)))
     gpu.sync()
     assert torch.equal(out, x[0]) and int(picks[0]) == int(x.argmax())
+
+
+def test_packed_rows_end_with_the_memory_of_x(gpu):
+    # x is rows in memory: what counts is what lies behind its first element, not its shape.
+    p = gpu.pass_()
+    pool = torch.zeros(2, 2, 1, 16, 8, dtype=torch.float16, device="cuda")
+    slots = i32([3, 20, 7])
+    row = torch.randn(16, device="cuda")
+    with pytest.raises(ValueError, match="fewer rows"):
+        p.pack_slots(row.expand(3, 16), (0, 16), slots, pool)
+    with pytest.raises(ValueError, match="fewer rows"):
+        p.pack_slots(torch.randn(3, 24, device="cuda")[:, ::2], (20, 24), slots, pool)
+    for before in (-1, 24):
+        with pytest.raises(ValueError, match="fewer rows"):
+            p.pack_slots(torch.randn(3, 24, device="cuda"), (before, 24 if before < 0 else -8), slots, pool)
+    x = torch.randn(3, 24, device="cuda")
+    p.pack_slots(x[:, 8:], (0, 24), slots, pool)  # a view whose last row ends with x
+    gpu.sync()
+    for r, s in enumerate([3, 20, 7]):
+        assert torch.equal(pool[s // 16, :, 0, s % 16].flatten(), x[r, 8:].half())

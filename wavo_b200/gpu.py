@@ -462,7 +462,10 @@ class Pass:
         cache, blocks, kv_heads, bs, hd = _pool(pool)
         src, stride = src_stride
         rows = slots.numel()
-        if rows and src + (rows - 1) * stride + 2 * kv_heads * hd > x.numel():
+        # Elements of memory from x's first one on.
+        room = x.numel() if x.is_contiguous() else \
+            x.untyped_storage().nbytes() // x.element_size() - x.storage_offset()
+        if rows and (min(src, stride) < 0 or src + (rows - 1) * stride + 2 * kv_heads * hd > room):
             raise ValueError("pack_slots: x has fewer rows")
         status = L.lib().wavo_pack_slots(self.ctx, _ptr(x), _dtype(x), src, stride, _i32(slots), rows,
                                          cache, blocks, bs, kv_heads, hd)
