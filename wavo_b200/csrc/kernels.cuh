@@ -240,6 +240,7 @@ struct AttendTreeArgs {
 // positions each. map: as below, boxes of min(bs, 64) positions.
 struct AttendFewPlan {
   int splits, chunk;
+  int most;  // splits of a call with these arguments and any shorter max_len, at most
 };
 AttendFewPlan attend_few_plan(int n, int max_rows, int max_len, int heads, int kv_heads, int hd,
                               int sms);

@@ -544,7 +544,7 @@ AttendFewPlan attend_few_plan(int n, int max_rows, int max_len, int heads, int k
   const long long slots = (hd <= 64 ? 3ll : 2ll) * sms;
   const long long want = std::max<long long>(1, slots / ctas);
   const long long most = std::max<long long>(1, (max_len + 255) / 256);
-  p.splits = int(std::min<long long>(std::min(want, most), 128));
+  p.splits = p.most = int(std::min<long long>(std::min(want, most), 128));
   p.chunk = int(((long long)max_len + p.splits - 1) / p.splits);
   p.chunk = std::max((p.chunk + TF_KEYS - 1) / TF_KEYS, 1) * TF_KEYS;
   p.splits = std::max((max_len + p.chunk - 1) / p.chunk, 1);

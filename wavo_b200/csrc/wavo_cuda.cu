@@ -1726,12 +1726,12 @@ size_t wavo_attend_tree_scratch(const wavo_ctx *ctx, uint32_t n, uint32_t rows, 
       max_len > 0x7fffffffu || n > 65535)
     return 0;
   // Of both kernels: which one a call takes, and its ranges, follow from the positions that its
-  // tables reach, max_len at most.
+  // tables reach, max_len at most. Fewer positions can make more ranges (their length is rounded).
+  wv::AttendFewPlan plan = wv::attend_few_plan(int(n), int(std::min(max_rows, rows)), int(max_len),
+                                               int(heads), int(kv_heads), int(hd), ctx->sms);
+  plan.splits = plan.most;
   return std::max(wv::attend_tree_part_bytes(int(hd), ctx->sms),
-                  wv::attend_few_part_bytes(
-                      wv::attend_few_plan(int(n), int(max_rows), int(max_len), int(heads),
-                                          int(kv_heads), int(hd), ctx->sms),
-                      int(rows), int(heads), int(hd)));
+                  wv::attend_few_part_bytes(plan, int(rows), int(heads), int(hd)));
 }
 
 wavo_status wavo_shape_logits(wavo_ctx *ctx, const void *logits, int dtype, uint64_t ld, void *out,
