@@ -1,0 +1,59 @@
+"""What TreeDecoder refuses and gives back on the GPU: prompts, segments that are done, the end of the
+context, another stream."""
+
+import numpy as np
+import pytest
+import torch
+
+import test_gpu_tree_decoder as D
+
+pytestmark = pytest.mark.gpu
+
+PROMPTS = [[3, 7, 11], [5], [9, 2, 2, 8, 1, 4]]
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    from wavo_b200.gpu import Gpu
+    g = Gpu(0)
+    yield g
+    g.close()
+
+
+@pytest.fixture(scope="module")
+def weights():
+    return D.encode(D.weights(np.random.default_rng(5)))
+
+
+def decoder(gpu, weights, batch=3, max_rows=24, context=D.CONTEXT, blocks=0):
+    from wavo_b200 import GGML_F16
+    from wavo_b200.blocks import TreeDecoder
+    dec = TreeDecoder(gpu, GGML_F16, D.D, D.HEADS, D.D_FF, D.VOCAB, context, D.FRAMES, batch, weights,
+                      max_rows, blocks=blocks)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    enc = torch.randn(batch, D.FRAMES, D.D, generator=g, device="cuda")
+    dec.record_cross(gpu.pass_(), enc)
+    return dec
+
+
+def steps(gpu, dec, last, n):
+    """n single-token steps from the last tokens: each segment's tokens."""
+    got = [[] for _ in last]
+    for _ in range(n):
+        for b, more in enumerate(dec.verify(gpu.pass_(), [([t], [-1]) for t in last])):
+            got[b] += more
+        last = [g[-1] for g in got]
+    return got
+
+
+def test_a_start_that_is_refused_leaves_the_windows(gpu, weights):
+    dec = decoder(gpu, weights)
+    want = steps(gpu, dec, dec.start(gpu.pass_(), PROMPTS), 6)
+    first = dec.start(gpu.pass_(), PROMPTS)
+    got = steps(gpu, dec, first, 2)
+    for bad in ([[1], [2], [D.VOCAB]], [[1], [2]], [[1], [2], list(range(25))]):
+        with pytest.raises(ValueError):
+            dec.start(gpu.pass_(), bad)
+    for b, more in enumerate(steps(gpu, dec, [g[-1] for g in got], 4)):
+        assert got[b] + more == want[b]

@@ -539,8 +539,8 @@ class TreeDecoder:
         p.gemm(y, self.embed, self.logits, rows, "bias")
         p.shape_logits(self.logits[:rows], self.rules, self.picks, self.logprobs)
 
-    def _load(self, trees) -> tuple[int, int]:
-        """The step's rows onto the device; (rows, the most of a segment)."""
+    def _check(self, trees):
+        """What `_load` takes, from trees that a step can run."""
         if len(trees) != self.batch:
             raise ValueError(f"{len(trees)} trees for {self.batch} segments")
         made = [([], []) if t is None else t for t in trees]
@@ -561,8 +561,13 @@ class TreeDecoder:
                 words[at:at + c, :m.shape[1]], depth[at:at + c] = m, dep
                 at += c
         adds = [-1 if t is None else c for t, c in zip(trees, counts)]
-        for to, a in ((self.adds, adds), (self.tokens[:rows], [x for t, _ in made for x in t]),
-                      (self.depth[:rows], depth), (self.mask[:rows], words)):
+        return rows, most, adds, [x for t, _ in made for x in t], depth, words
+
+    def _load(self, step) -> tuple[int, int]:
+        """The step's rows onto the device; (rows, the most of a segment)."""
+        rows, most, adds, tokens, depth, words = step
+        for to, a in ((self.adds, adds), (self.tokens[:rows], tokens), (self.depth[:rows], depth),
+                      (self.mask[:rows], words)):
             to.copy_(torch.as_tensor(np.asarray(a, np.int32)))
         return rows, most
 
@@ -587,6 +592,7 @@ class TreeDecoder:
     def start(self, p: Pass, prompts) -> list[int]:
         """A new window: each segment's prompt tokens into its cache. Returns each segment's first
         token. Segments that are under way give their blocks back."""
+        step = self._check([(list(t), list(range(-1, len(t) - 1))) for t in prompts])
         self.adds.fill_(-1)
         none = self.row_seq[:0]
         p.block_tables(self.lens, self.adds, self.bs, self.ring, self.state, self.owned, self.table,
@@ -594,7 +600,7 @@ class TreeDecoder:
         self.state.copy_(self.state_next[:2])
         self.owned.copy_(self.owned_next)
         self.lens.zero_()
-        rows, most = self._load([(list(t), list(range(-1, len(t) - 1))) for t in prompts])
+        rows, most = self._load(step)
         self._record(p, rows, most)
         self._refused()
         counts = self.adds.clone()
@@ -610,7 +616,7 @@ class TreeDecoder:
         gives its blocks back. Returns the tokens each segment gains: the drafted ones that greedy decoding
         gives too, and the one after them (none for a segment that is done; -1 where the rules leave
         no token)."""
-        rows, most = self._load(trees)
+        rows, most = self._load(self._check(trees))
         if rows == 0:
             return [[] for _ in trees]
         self._record(p, rows, most)
