@@ -57,3 +57,13 @@ def test_a_start_that_is_refused_leaves_the_windows(gpu, weights):
             dec.start(gpu.pass_(), bad)
     for b, more in enumerate(steps(gpu, dec, [g[-1] for g in got], 4)):
         assert got[b] + more == want[b]
+
+
+@pytest.mark.parametrize("at", [0, 1, 2])
+def test_a_prompt_without_tokens_is_refused(gpu, weights, at):
+    # It has no last row, whose pick would be the segment's first token.
+    dec = decoder(gpu, weights)
+    prompts = [list(t) for t in PROMPTS]
+    prompts[at] = []
+    with pytest.raises(ValueError, match="prompt"):
+        dec.start(gpu.pass_(), prompts)

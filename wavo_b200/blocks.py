@@ -590,9 +590,11 @@ class TreeDecoder:
             raise RuntimeError(f"{short} segments have no blocks left: give a larger `blocks`")
 
     def start(self, p: Pass, prompts) -> list[int]:
-        """A new window: each segment's prompt tokens into its cache. Returns each segment's first
+        """A new window: each segment's prompt tokens (one at least) into its cache. Returns each segment's first
         token. Segments that are under way give their blocks back."""
         step = self._check([(list(t), list(range(-1, len(t) - 1))) for t in prompts])
+        if not all(step[2]):
+            raise ValueError("a prompt without tokens")
         self.adds.fill_(-1)
         none = self.row_seq[:0]
         p.block_tables(self.lens, self.adds, self.bs, self.ring, self.state, self.owned, self.table,
