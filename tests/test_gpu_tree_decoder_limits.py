@@ -67,3 +67,22 @@ def test_a_prompt_without_tokens_is_refused(gpu, weights, at):
     prompts[at] = []
     with pytest.raises(ValueError, match="prompt"):
         dec.start(gpu.pass_(), prompts)
+
+
+def test_blocks_come_back_when_every_segment_is_done(gpu, weights):
+    dec = decoder(gpu, weights)
+    blocks = int(dec.state[1])
+    steps(gpu, dec, dec.start(gpu.pass_(), PROMPTS), 3)
+    assert int(dec.state[1]) < blocks
+    assert dec.verify(gpu.pass_(), [None] * 3) == [[]] * 3
+    assert int(dec.state[1]) == blocks
+    assert dec.owned.tolist() == [0] * 3
+    # Again, and beside segments that wait.
+    assert dec.verify(gpu.pass_(), [None] * 3) == [[]] * 3
+    first = dec.start(gpu.pass_(), PROMPTS)
+    assert dec.verify(gpu.pass_(), [None, ([], []), None]) == [[]] * 3
+    assert int(dec.state[1]) == blocks - 1
+    got = dec.verify(gpu.pass_(), [None, ([first[1]], [-1]), None])
+    assert [len(g) for g in got] == [0, 1, 0] and int(dec.state[1]) == blocks - 1
+    dec.start(gpu.pass_(), PROMPTS)
+    assert int(dec.state[1]) == blocks - 3

@@ -589,6 +589,14 @@ class TreeDecoder:
         if short:
             raise RuntimeError(f"{short} segments have no blocks left: give a larger `blocks`")
 
+    def _give_back(self, p: Pass) -> None:
+        """The plan of a step without rows: the segments that are done give their blocks back."""
+        none = self.row_seq[:0]
+        p.block_tables(self.lens, self.adds, self.bs, self.ring, self.state, self.owned, self.table,
+                       self.row_start, none, none, self.state_next, self.owned_next)
+        self.state.copy_(self.state_next[:2])
+        self.owned, self.owned_next = self.owned_next, self.owned
+
     def start(self, p: Pass, prompts) -> list[int]:
         """A new window: each segment's prompt tokens (one at least) into its cache. Returns each segment's first
         token. Segments that are under way give their blocks back."""
@@ -596,11 +604,7 @@ class TreeDecoder:
         if not all(step[2]):
             raise ValueError("a prompt without tokens")
         self.adds.fill_(-1)
-        none = self.row_seq[:0]
-        p.block_tables(self.lens, self.adds, self.bs, self.ring, self.state, self.owned, self.table,
-                       self.row_start, none, none, self.state_next, self.owned_next)
-        self.state.copy_(self.state_next[:2])
-        self.owned.copy_(self.owned_next)
+        self._give_back(p)
         self.lens.zero_()
         rows, most = self._load(step)
         self._record(p, rows, most)
@@ -620,6 +624,7 @@ class TreeDecoder:
         no token)."""
         rows, most = self._load(self._check(trees))
         if rows == 0:
+            self._give_back(p)
             return [[] for _ in trees]
         self._record(p, rows, most)
         self._refused()  # before the commit, so that the caches are those of the step before
