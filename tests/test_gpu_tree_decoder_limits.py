@@ -86,3 +86,19 @@ def test_blocks_come_back_when_every_segment_is_done(gpu, weights):
     assert [len(g) for g in got] == [0, 1, 0] and int(dec.state[1]) == blocks - 1
     dec.start(gpu.pass_(), PROMPTS)
     assert int(dec.state[1]) == blocks - 3
+
+
+@pytest.mark.parametrize("together", [True, False])
+def test_a_segment_that_is_done_holds_nothing(gpu, weights, together):
+    # What comes for it next begins an empty window, with blocks of its own from then on.
+    dec = decoder(gpu, weights)
+    blocks = int(dec.state[1])
+    want = steps(gpu, dec, [7, 8, 9], 5)
+    dec = decoder(gpu, weights)
+    first = dec.start(gpu.pass_(), [[4] * 20, [5] * 20, [6] * 20])
+    dec.verify(gpu.pass_(), [None] * 3 if together else [None, ([first[1]], [-1]), None])
+    dec.verify(gpu.pass_(), [([], [])] * 3)
+    assert int(dec.state[1]) == blocks - (0 if together else 2)
+    dec.verify(gpu.pass_(), [([], []), None, ([], [])])
+    assert int(dec.state[1]) == blocks and dec.lens.tolist() == [0] * 3
+    assert steps(gpu, dec, [7, 8, 9], 5) == want

@@ -590,12 +590,14 @@ class TreeDecoder:
             raise RuntimeError(f"{short} segments have no blocks left: give a larger `blocks`")
 
     def _give_back(self, p: Pass) -> None:
-        """The plan of a step without rows: the segments that are done give their blocks back."""
+        """The plan of a step without rows: the segments that are done give their blocks back, and
+        hold no position from then on."""
         none = self.row_seq[:0]
         p.block_tables(self.lens, self.adds, self.bs, self.ring, self.state, self.owned, self.table,
                        self.row_start, none, none, self.state_next, self.owned_next)
         self.state.copy_(self.state_next[:2])
         self.owned, self.owned_next = self.owned_next, self.owned
+        self.lens.masked_fill_(self.adds < 0, 0)
 
     def start(self, p: Pass, prompts) -> list[int]:
         """A new window: each segment's prompt tokens (one at least) into its cache. Returns each segment's first
@@ -605,7 +607,6 @@ class TreeDecoder:
             raise ValueError("a prompt without tokens")
         self.adds.fill_(-1)
         self._give_back(p)
-        self.lens.zero_()
         rows, most = self._load(step)
         self._record(p, rows, most)
         self._refused()
@@ -618,10 +619,10 @@ class TreeDecoder:
 
     def verify(self, p: Pass, trees) -> list[list[int]]:
         """One step. trees[b]: (tokens, parents) of segment b, tokens[0] its last decided token (parent
-        -1), the others drafted continuations, parents before children; None: the segment is done and
-        gives its blocks back. Returns the tokens each segment gains: the drafted ones that greedy decoding
-        gives too, and the one after them (none for a segment that is done; -1 where the rules leave
-        no token)."""
+        -1), the others drafted continuations, parents before children; None: the segment is done,
+        gives its blocks back and holds nothing. Returns the tokens each segment gains: the drafted ones
+        that greedy decoding gives too, and the one after them (none for a segment that is done; -1
+        where the rules leave no token)."""
         rows, most = self._load(self._check(trees))
         if rows == 0:
             self._give_back(p)
@@ -630,6 +631,7 @@ class TreeDecoder:
         self._refused()  # before the commit, so that the caches are those of the step before
         p.tree_accept(self.picks, self.tokens[:rows], self.mask[:rows], self.row_start, self.lens,
                       self.table, self.pool, self.path, self.count, self.next, self.lens_next)
+        self.lens_next.masked_fill_(self.adds < 0, 0)
         out = torch.cat([self.path, self.count[:, None], self.next[:, None]], 1).tolist()
         self._keep(self.count, self.row_start[:-1, None] + self.path)
         gained = []
