@@ -102,3 +102,37 @@ def test_a_segment_that_is_done_holds_nothing(gpu, weights, together):
     dec.verify(gpu.pass_(), [([], []), None, ([], [])])
     assert int(dec.state[1]) == blocks and dec.lens.tolist() == [0] * 3
     assert steps(gpu, dec, [7, 8, 9], 5) == want
+
+
+def test_the_end_of_the_context(gpu, weights):
+    # A segment gains the tokens that its positions give, one after the last of them included, drafts
+    # or not, and is then refused with that reason.
+    context = 20
+    full = decoder(gpu, weights)
+    want = []
+    first = full.start(gpu.pass_(), PROMPTS)
+    for t, p, more in zip(first, PROMPTS, steps(gpu, full, first, context)):
+        want.append([t, *more][:context - len(p) + 1])
+    for drafts in (0, 1, 4, 30):
+        dec = decoder(gpu, weights, context=context, max_rows=31)
+        got = [[t] for t in dec.start(gpu.pass_(), PROMPTS)]
+        assert [g[0] for g in got] == first
+        for _ in range(context):
+            trees = []
+            for g, w in zip(got, want):
+                # Right drafts to the end of what there is, then wrong ones.
+                chain = (w[len(g):] + [1] * 30)[:drafts]
+                trees.append(None if len(g) == len(w) else ([g[-1]] + chain, list(range(-1, len(chain)))))
+            if trees == [None] * 3:
+                break
+            for g, more in zip(got, dec.verify(gpu.pass_(), trees)):
+                g += more
+        assert got == want
+        assert dec.verify(gpu.pass_(), [None] * 3) == [[]] * 3
+    dec = decoder(gpu, weights, context=context)
+    first = dec.start(gpu.pass_(), [[4] * context, [5], [6]])
+    with pytest.raises(ValueError, match="context"):
+        dec.verify(gpu.pass_(), [([t], [-1]) for t in first])
+    assert dec.verify(gpu.pass_(), [None] + [([t], [-1]) for t in first[1:]])[0] == []
+    with pytest.raises(ValueError, match="context"):
+        dec.start(gpu.pass_(), [[4] * (context + 1), [5], [6]])

@@ -458,6 +458,7 @@ class TreeDecoder:
         self.owned, self.owned_next = i32(batch), i32(batch)
         self.lens, self.lens_next = i32(batch), i32(batch)
         self.state[1] = blocks
+        self.held = [0] * batch  # lens, as the host knows them
         # The encoder's K and V: planned once, full blocks of a segment's frames.
         cross = -(-frames // bs)
         self.cross = f16(n_layers, batch * cross, 2, heads, bs, self.hd)
@@ -539,8 +540,8 @@ class TreeDecoder:
         p.gemm(y, self.embed, self.logits, rows, "bias")
         p.shape_logits(self.logits[:rows], self.rules, self.picks, self.logprobs)
 
-    def _check(self, trees):
-        """What `_load` takes, from trees that a step can run."""
+    def _check(self, trees, held):
+        """What `_load` takes, from trees that a step can run on segments of `held` positions."""
         if len(trees) != self.batch:
             raise ValueError(f"{len(trees)} trees for {self.batch} segments")
         made = [([], []) if t is None else t for t in trees]
@@ -548,6 +549,9 @@ class TreeDecoder:
         most, rows = max(counts), sum(counts)
         if most > self.max_rows:
             raise ValueError(f"{most} rows of a segment (at most {self.max_rows})")
+        for b, (c, n) in enumerate(zip(counts, held)):
+            if c and n >= self.context:
+                raise ValueError(f"segment {b} fills its context of {self.context} positions")
         words = np.zeros((rows, self.mask.shape[1]), np.int32)
         depth = np.zeros(rows, np.int32)
         at = 0
@@ -602,9 +606,10 @@ class TreeDecoder:
     def start(self, p: Pass, prompts) -> list[int]:
         """A new window: each segment's prompt tokens (one at least) into its cache. Returns each segment's first
         token. Segments that are under way give their blocks back."""
-        step = self._check([(list(t), list(range(-1, len(t) - 1))) for t in prompts])
-        if not all(step[2]):
-            raise ValueError("a prompt without tokens")
+        step = self._check([(list(t), list(range(-1, len(t) - 1))) for t in prompts], [0] * self.batch)
+        if not all(0 < n <= self.context for n in step[2]):
+            raise ValueError(f"a prompt without tokens or past the context of {self.context} positions")
+        self.held = [0] * self.batch
         self.adds.fill_(-1)
         self._give_back(p)
         rows, most = self._load(step)
@@ -613,6 +618,7 @@ class TreeDecoder:
         counts = self.adds.clone()
         torch.add(self.lens, counts, out=self.lens_next)
         i = torch.arange(most, dtype=torch.int32, device=counts.device)
+        self.held = step[2]
         last = self.picks[(self.row_start[1:] - 1).long()].tolist()
         self._keep(counts, self.row_start[:-1, None] + i)
         return last
@@ -622,19 +628,28 @@ class TreeDecoder:
         -1), the others drafted continuations, parents before children; None: the segment is done,
         gives its blocks back and holds nothing. Returns the tokens each segment gains: the drafted ones
         that greedy decoding gives too, and the one after them (none for a segment that is done; -1
-        where the rules leave no token)."""
-        rows, most = self._load(self._check(trees))
+        where the rules leave no token). Drafts past the context are not kept, and a segment that
+        fills it cannot go on (ValueError)."""
+        step = self._check(trees, self.held)
+        rows, most = self._load(step)
         if rows == 0:
             self._give_back(p)
+            self.held = [0 if t is None else n for t, n in zip(trees, self.held)]
             return [[] for _ in trees]
         self._record(p, rows, most)
         self._refused()  # before the commit, so that the caches are those of the step before
         p.tree_accept(self.picks, self.tokens[:rows], self.mask[:rows], self.row_start, self.lens,
                       self.table, self.pool, self.path, self.count, self.next, self.lens_next)
+        # What lies past the context was embedded as its last position and is not kept.
+        self.lens_next.clamp_(max=self.context)
+        kept = self.lens_next - self.lens
         self.lens_next.masked_fill_(self.adds < 0, 0)
-        out = torch.cat([self.path, self.count[:, None], self.next[:, None]], 1).tolist()
-        self._keep(self.count, self.row_start[:-1, None] + self.path)
+        out = torch.cat([self.path, self.count[:, None], self.next[:, None], self.lens_next[:, None]],
+                        1).tolist()
+        self._keep(kept, self.row_start[:-1, None] + self.path)
         gained = []
-        for t, (*path, count, after) in zip(trees, out):
-            gained.append([] if t is None or not count else [t[0][i] for i in path[1:count]] + [after])
+        for b, (t, (*path, count, after, held)) in enumerate(zip(trees, out)):
+            said = [] if t is None or not count else [t[0][i] for i in path[1:count]] + [after]
+            gained.append(said[:held - self.held[b]] if said else said)
+            self.held[b] = held
         return gained
