@@ -33,6 +33,7 @@ def decoder(gpu, weights, batch=3, max_rows=24, context=D.CONTEXT, blocks=0):
     g = torch.Generator(device="cuda")
     g.manual_seed(1)
     enc = torch.randn(batch, D.FRAMES, D.D, generator=g, device="cuda")
+    torch.cuda.current_stream().synchronize()  # (the encoder's output may come from another stream)
     dec.record_cross(gpu.pass_(), enc)
     return dec
 
@@ -136,3 +137,40 @@ def test_the_end_of_the_context(gpu, weights):
     assert dec.verify(gpu.pass_(), [None] + [([t], [-1]) for t in first[1:]])[0] == []
     with pytest.raises(ValueError, match="context"):
         dec.start(gpu.pass_(), [[4] * (context + 1), [5], [6]])
+
+
+@pytest.mark.parametrize("how", ["context", "torch"])
+def test_a_step_runs_on_the_contexts_stream(gpu, weights, how):
+    # The library's work and torch's of a step are on one stream, whichever is torch's current one,
+    # which is kept busy here.
+    dec = decoder(gpu, weights)
+    want = steps(gpu, dec, dec.start(gpu.pass_(), PROMPTS), 4)
+    torch.cuda.synchronize()
+    side, here = torch.cuda.Stream(), torch.cuda.current_stream()
+
+    def busy():
+        torch.cuda._sleep(20_000_000)  # some 10 ms
+
+    def go():
+        busy()
+        dec = decoder(gpu, weights)
+        busy()
+        last, got = dec.start(gpu.pass_(), PROMPTS), [[] for _ in PROMPTS]
+        for _ in range(4):
+            busy()
+            for g, more in zip(got, steps(gpu, dec, last, 1)):
+                g += more
+            last = [g[-1] for g in got]
+        return got
+    if how == "context":
+        gpu.use_stream(side)
+        try:
+            got = go()
+        finally:
+            side.synchronize()
+            gpu.use_stream(here)
+    else:
+        with torch.cuda.stream(side):
+            got = go()
+    torch.cuda.synchronize()
+    assert got == want

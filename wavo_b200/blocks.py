@@ -12,6 +12,7 @@ projection reads; the output projection adds into the caller's f32 residual stre
 
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -410,6 +411,16 @@ def tree_masks(parents) -> tuple[np.ndarray, np.ndarray]:
     return words.view(np.int32), depth
 
 
+def _on_stream(method):
+    """torch's work of a method on the context's stream, in order with the library's."""
+    @functools.wraps(method)
+    def run(self, *args, **kw):
+        gpu = getattr(self, "gpu", None) or kw.get("gpu") or args[0]  # (the constructor's first)
+        with torch.cuda.stream(gpu.stream):
+            return method(self, *args, **kw)
+    return run
+
+
 class TreeDecoder:
     """The Whisper decoder over paged caches, verifying several drafted tokens a segment in one step
     (no reference counterpart: the reference decodes a token a step, src/transformer.rs:254-290, which
@@ -425,6 +436,7 @@ class TreeDecoder:
     segments: penalties (repetition, presence, frequency), bias {token: value}, allowed (a bool array of
     the vocabulary, e.g. without the timestamps and Whisper's suppressed tokens)."""
 
+    @_on_stream
     def __init__(self, gpu: Gpu, ty: int, d: int, heads: int, d_ff: int, vocab: int, context: int,
                  frames: int, batch: int, w: dict, max_rows: int, bs: int = 16, blocks: int = 0,
                  penalties=None, bias=None, allowed=None):
@@ -498,6 +510,7 @@ class TreeDecoder:
             grammar=grammar, tree=(self.row_seq, self.row_start, self.tokens, self.mask))
         self.rules, self.rules_next = rule(self.lens), rule(self.lens_next)
 
+    @_on_stream
     def record_cross(self, p: Pass, enc: torch.Tensor, chunk: int = 8) -> None:
         """The encoder's K and V of every layer from its output [batch][frames][d] (f16 or f32);
         chunk segments a projection."""
@@ -603,6 +616,7 @@ class TreeDecoder:
         self.owned, self.owned_next = self.owned_next, self.owned
         self.lens.masked_fill_(self.adds < 0, 0)
 
+    @_on_stream
     def start(self, p: Pass, prompts) -> list[int]:
         """A new window: each segment's prompt tokens (one at least) into its cache. Returns each segment's first
         token. Segments that are under way give their blocks back."""
@@ -623,6 +637,7 @@ class TreeDecoder:
         self._keep(counts, self.row_start[:-1, None] + i)
         return last
 
+    @_on_stream
     def verify(self, p: Pass, trees) -> list[list[int]]:
         """One step. trees[b]: (tokens, parents) of segment b, tokens[0] its last decided token (parent
         -1), the others drafted continuations, parents before children; None: the segment is done,

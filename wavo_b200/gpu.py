@@ -158,6 +158,7 @@ class Gpu:
 
     def use_stream(self, stream: torch.cuda.Stream) -> None:
         check(L.lib().wavo_set_stream(self.ctx, stream.cuda_stream), self.ctx)
+        self.stream = stream
 
     def close(self) -> None:
         if L is None or L.lib is None:  # interpreter shutdown: the process releases the device
