@@ -116,3 +116,95 @@ def test_items_that_end_inside_a_run_over_and_over(gpu, dtype, heads, kvh, hd):
     got = attend(gpu, q, pool, table, starts, lens, mask, counts, times=60)
     want, terms = attend64(q, pool, table, starts, lens, mask, heads)
     hold(got, want, terms, dtype)
+
+
+SHAPES = [(16, 2, 64), (16, 2, 128), (24, 2, 40)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kvh,hd", SHAPES)
+def test_many_short_items_a_run(gpu, dtype, heads, kvh, hd):
+    # Several hundred requests of one to four tiles, one or two items a K and V head: a run has more
+    # items than the kernel holds at a time. Some have no rows, no positions, or neither.
+    rng = np.random.default_rng(hd + 1)
+    n = 420
+    lens = rng.integers(0, 480, n)
+    counts = rng.integers(1, 21, n)
+    lens[rng.random(n) < 0.1] = 0
+    counts[rng.random(n) < 0.1] = 0
+    counts[0], counts[1] = 20, 0
+    lens, counts = lens.tolist(), counts.tolist()
+    q, pool, table, starts, mask = make(hd, dtype, counts, lens, heads, kvh, hd, 16)
+    mask[rng.random(len(mask)) < 0.05] = 0  # rows that see no drafted position
+    got = attend(gpu, q, pool, table, starts, lens, mask, counts, times=5)
+    want, terms = attend64(q, pool, table, starts, lens, mask, heads)
+    hold(got, want, terms, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kvh,hd", SHAPES)
+@pytest.mark.parametrize("tree", [True, False])
+def test_many_tiles_a_run(gpu, dtype, heads, kvh, hd, tree):
+    # Few long items: a run has more than ten tiles of one, and every item spans many runs.
+    counts, lens = [20, 9], [70001, 52345]
+    q, pool, table, starts, mask = make(hd, dtype, counts, lens, heads, kvh, hd, 64, tree)
+    got = attend(gpu, q, pool, table, starts, lens, mask, counts, times=5)
+    want, terms = attend64(q, pool, table, starts, lens, mask, heads)
+    hold(got, want, terms, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kvh,hd", SHAPES)
+def test_scores_that_rise_late(gpu, dtype, heads, kvh, hd):
+    # K grows towards a request's end, in steps of its own for every K and V head: the references
+    # rise, and the outputs so far are scaled, at tiles anywhere in a run.
+    rng = np.random.default_rng(hd + 2)
+    lens = rng.integers(1400, 6000, 12).tolist()
+    counts = rng.integers(9, 21, 12).tolist()
+    q, pool, table, starts, mask = make(hd, dtype, counts, lens, heads, kvh, hd, 16)
+    for s, (n, c) in enumerate(zip(lens, counts)):
+        for b in range((n + c) // 16):
+            grown = 0.2 + 4 * (b * 16 / n) ** (1 + np.arange(kvh) * 3)
+            pool[int(table[s, b]), 0] *= torch.as_tensor(grown).cuda().half()[:, None, None]
+    got = attend(gpu, q, pool, table, starts, lens, mask, counts, times=3)
+    want, terms = attend64(q, pool, table, starts, lens, mask, heads)
+    hold(got, want, terms, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,kvh,hd", SHAPES)
+@pytest.mark.parametrize("long", [False, True])
+def test_infinities_in_one_item_after_another(gpu, dtype, heads, kvh, hd, long):
+    # Drafted rows of most requests hold infinities and NaN in V, each in elements of its own: rows
+    # that see one get it there, and nowhere else.
+    rng = np.random.default_rng(hd + 3)
+    n = 10 if long else 200
+    lens = rng.integers(1400, 4000, n) if long else rng.integers(0, 400, n)
+    counts = rng.integers(8, 21, n)
+    counts[0] = 20
+    lens, counts = lens.tolist(), counts.tolist()
+    q, pool, table, starts, mask = make(hd, dtype, counts, lens, heads, kvh, hd, 16)
+    clean = pool.clone()
+    kinds = np.array([np.nan, np.inf, -np.inf])
+    odd = np.zeros((sum(counts), kvh, hd))  # what the drafted rows hold, 0 where it is finite
+    for s, (ln, c) in enumerate(zip(lens, counts)):
+        for j in rng.choice(c, 2, replace=False) if rng.random() < 0.8 else []:
+            for h in range(kvh):
+                e = int(rng.integers(0, hd))
+                odd[starts[s] + j, h, e] = rng.choice(kinds)
+                at = int(table[s, (ln + j) // 16]), (ln + j) % 16
+                pool[at[0], 1, h, at[1], e] = odd[starts[s] + j, h, e]
+                clean[at[0], 1, h, at[1], e] = 0
+    got = attend(gpu, q, pool, table, starts, lens, mask, counts).double().cpu().numpy()
+    want, terms = attend64(q, clean, table, starts, lens, mask, heads)
+    for s, c in enumerate(counts):
+        for r in range(starts[s], starts[s + 1]):
+            for j in range(c):
+                if R.sees(mask[r], j):
+                    add = np.repeat(odd[starts[s] + j], heads // kvh, 0).reshape(-1)
+                    with np.errstate(invalid="ignore"):
+                        want[r] += add
+    whole = np.isfinite(want)
+    assert (~whole).any() and np.array_equal(got[~whole], want[~whole], equal_nan=True)
+    bound = R.attend_bound(want, terms, dtype == "f16")
+    assert (np.abs(got[whole] - want[whole]) <= bound[whole]).all()
