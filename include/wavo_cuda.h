@@ -383,7 +383,7 @@ wavo_status wavo_pack_slots(wavo_ctx *ctx, const void *x, int x_dtype, uint32_t 
  * lens[s] + j of the rows j < the request's whose bit is set; any bits may be set. mask NULL: the
  * lens[s] positions alone (a single token whose K and V are packed already, or the queries of a
  * cross attention over the encoder frames). row_start NULL: request s has the one row s. Head h reads
- * K and V head h / (heads / kv_heads). max_rows is at least the rows of every request (at most
+ * K and V head h / (heads / kv_heads). n and the heads are 65535 at most. max_rows is at least the rows of every request (at most
  * 32 * mask_words with a mask), max_len at least every number of positions, cached and drafted
  * (what lies beyond is not seen). Scores are scaled by 1 / sqrt(hd). A row that sees nothing gets
  * zeros; what a row does not see has no effect on it, whatever it holds. WAVO_F16: f16 products,
@@ -392,7 +392,8 @@ wavo_status wavo_pack_slots(wavo_ctx *ctx, const void *x, int x_dtype, uint32_t 
  * the probabilities to 2^-22 of each down to the same 2^-25, q (below f16's largest value) to 2^-22
  * or 2^-25, whichever is more. Measured against 64 bits: relative 2-norms of 2e-7 to 3e-6, growing
  * with the positions. Table entries outside the pool are positions that no row sees.
- * wavo_attend_tree_scratch is the scratch that a call needs (see wavo_reserve). */
+ * wavo_attend_tree_scratch is the scratch that a call needs, also with a shorter max_len (see
+ * wavo_reserve). */
 wavo_status wavo_attend_tree(wavo_ctx *ctx, const void *q, uint64_t q_stride, int dtype,
                              const void *pool, uint32_t blocks, uint32_t bs, const int32_t *table,
                              uint32_t width, const int32_t *row_start, const int32_t *lens,

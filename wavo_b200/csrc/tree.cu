@@ -20,9 +20,10 @@
 // its part in global memory, and a second kernel joins an item's parts in the order of the runs.
 //
 // Two requests of up to 131072 positions, 8 K and V heads of 128 and up to 96 rows each (685 MB, 53
-// GFLOP): 143 us and 9 for the join, 4.8 TB/s; the loads alone, in the same runs, take 137 to 157.
-// A tile costs the softmax warps about 2300 cycles (the exponentials 770 of them) and its 64 KB an
-// SM's share of the memory 2800; at the clocks that the power limit leaves the two are close.
+// GFLOP): a pass by itself 144 us and 9 for the join, 4.5 TB/s; among other passes, at the clocks that
+// the power limit leaves, 166 us in all, 4.1 TB/s. The loads alone, in the same runs, took 137 to
+// 157. A tile costs the softmax warps about 2300 cycles (the exponentials 770 of them) and its 64 KB
+// an SM's share of the memory 2800; at the lower clocks the two are close.
 // Positions as the UMMA's M and the rows as its N (P through shared memory, a vote of all warps a
 // tile) took 215 us, the join by the last CTA alone 57 more.
 #include <algorithm>
@@ -800,11 +801,14 @@ cudaError_t launch_tile(const CUtensorMap &map, const AttendTreeArgs &a, int sms
 
 }  // namespace
 
-// Measured on both sides, us few : many, f16 and f32. Long: 2 x 16384 positions, heads of 128: 32
-// rows 38 : 38, 46 : 49; 48 rows 47 : 40, 62 : 53; 96 rows 70 : 53, 90 : 73; heads of 64: 32 rows
-// 43 : 53, 54 : 57; 48 rows 66 : 57, 99 : 65. 32 x 1500, heads of 64: 48 rows 95 : 87, 116 : 120;
-// 96 rows 135 : 102, 176 : 155. Short: 32 x 512, heads of 128: 64 rows 42 : 50, 48 : 74; 128 rows
-// 66 : 74, 93 : 96; 192 rows 117 : 76, 118 : 124; heads of 64: 96 rows 62 : 63, 72 : 149.
+// Measured on both sides, us few : many, f16 and f32, all requests with that many rows of a K and V
+// head and no mask. Long: 2 x 16384 positions, 8 K and V heads of 128: 32 rows 51 : 47, 58 : 57; 48
+// rows 53 : 49, 78 : 63; 96 rows 70 : 55, 104 : 80; heads of 64: 32 rows 39 : 37, 43 : 43; 48 rows
+// 39 : 37, 51 : 47. 32 x 1500, 20 heads of 64: 48 rows 104 : 90, 137 : 131; 96 rows 141 : 106,
+// 202 : 164. Trees of 1 to that many rows bring less work to CTAs of 32 rows, and the border lies
+// higher: 32 x 1500, 48 rows 86 : 94, 104 : 126; 96 rows 123 : 109, 174 : 167; 32 x 512, 8 heads of 128:
+// 64 rows 47 : 47, 63 : 68; 128 rows 74 : 68, 84 : 97; 192 rows 74 : 72, 115 : 113; 20 heads of 64: 96
+// rows 68 : 66, 96 : 112. The rule lies between the two: the host does not know the trees.
 bool attend_tree_few(int max_rows, int max_len, int heads, int kv_heads) {
   const long long rows = (long long)max_rows * (heads / kv_heads);
   return rows <= 32 || (rows <= 128 && max_len < 1280);

@@ -1,23 +1,24 @@
 // attend_tree for few rows: an item is one K and V head of one request with the rows that read it
 // (its drafted rows and the heads that share it), 32 at most in a CTA. The steps from a tile's
 // arrival to its sums are then short and the tiles of a request few, so what counts is how many of
-// them are under way at once: mma.sync with everything in registers between the products, no tensor
-// memory, no hand-over between warps, and 2 to 5 CTAs an SM. The form with tcgen05 (tree.cu) takes
-// over where the products would bound it; the figures of both are beside the rule there.
+// them are under way at once: mma.sync with the scores, probabilities and sums in registers, no tensor
+// memory, no hand-over between warps, and 2 to 5 CTAs an SM. (The f32 forms spill 8 to 17 words a
+// thread for that many.) The form with tcgen05 (tree.cu) takes over where the products would bound
+// it; the figures of both are beside the rule there.
 //
 // One pass over K and V with the softmax's running maximum and sum: a CTA takes an item's rows over
 // a range of positions. A producer warp loads 64 positions at a time, page by page, through TMA
 // boxes that follow the block table; four warps multiply, 16 rows each: they share a tile's
 // positions, and meet in shared memory at the end.
 //
-// Bound by the loads: 32 x 20 items of 16 rows over 1500 positions (246 MB, f16) take 46 us, 5.3
+// Bound by the loads: 32 x 20 items of 16 rows over 1500 positions (246 MB, f16) take 48 us, 5.2
 // TB/s; the same loads without the products took 54 us in CTAs of their own. One f32 row an item
-// over 448 positions at most (34 MB) 18 us, of which launch and the first page's way (row starts,
-// table, K) are most. Up to 64 f32 rows an item over 448 positions (two products each way) 47 us,
+// over 448 positions at most (34 MB) 19 us, of which launch and the first page's way (row starts,
+// table, K) are most. Up to 64 f32 rows an item over 448 positions (two products each way) 48 us,
 // bound by the latency of 16 warps an SM; 64 rows a CTA, a page read once, took 7 more (three CTAs
 // an SM), 16 rows a CTA as long, but 33 for 25 us where 32 rows have 1500 positions. Two stages and
 // five CTAs instead of three and four: 62 -> 50 us at the first; Q in shared memory, not registers:
-// 50 -> 46.
+// 50 -> 48. The scaling of f32's probabilities (split2_up) is 0.6 and 1.2 us of the two f32 figures.
 #include <algorithm>
 #include <type_traits>
 
@@ -540,7 +541,8 @@ AttendFewPlan attend_few_plan(int n, int max_rows, int max_len, int heads, int k
   AttendFewPlan p;
   const long long rows = (long long)max_rows * (heads / kv_heads);
   const long long ctas = (long long)n * kv_heads * ((rows + TF_ROWS - 1) / TF_ROWS);
-  // Ranges of 256 positions at least, as many as fill the SMs.
+  // Ranges of 256 positions at least, as many as fill the SMs with three CTAs each (two for heads of
+  // more than 64), also where an SM holds four or five.
   const long long slots = (hd <= 64 ? 3ll : 2ll) * sms;
   const long long want = std::max<long long>(1, slots / ctas);
   const long long most = std::max<long long>(1, (max_len + 255) / 256);
